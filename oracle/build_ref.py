@@ -60,7 +60,7 @@ def build(reference: str = DEFAULT_REFERENCE, force: bool = False) -> list[str]:
     """Build every module whose .so is missing or older than its source.
 
     Returns the list of built paths; returns [] without error when the
-    reference checkout is absent (e.g. on the GPU box).
+    reference checkout is absent or empty (e.g. on the GPU box).
     """
     if not os.path.isdir(reference):
         return []
@@ -68,6 +68,8 @@ def build(reference: str = DEFAULT_REFERENCE, force: bool = False) -> list[str]:
     for name, fname in MODULES.items():
         src = os.path.join(reference, fname)
         out = so_path(name)
+        if not os.path.exists(src):     # an empty or partial checkout
+            continue
         if not force and os.path.exists(out) and os.path.getmtime(out) >= os.path.getmtime(src):
             continue
         code = (f"import sys; sys.path.insert(0, {os.path.dirname(HERE)!r}); "
