@@ -14,6 +14,16 @@ from .build import LIB_PATH
 _c_int64 = ctypes.c_int64
 _vp = ctypes.c_void_p
 
+
+class PagedCache(ctypes.Structure):
+    """``ddq_paged_cache``: one pool of pages of keys and values."""
+    _fields_ = [("k", _vp), ("v", _vp), ("num_pages", _c_int64), ("page_size", _c_int64),
+                ("Hkv", _c_int64), ("D", _c_int64), ("page_stride", _c_int64),
+                ("head_stride", _c_int64), ("row_stride", _c_int64), ("dtype", ctypes.c_int)]
+
+
+_cache_p = ctypes.POINTER(PagedCache)
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "ddq_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -53,6 +63,23 @@ _SIGNATURES = {
     "ddq_lm_head_argmax": (ctypes.c_int, [_vp, _vp, _vp, _c_int64, _c_int64, _c_int64, _c_int64,
                                           _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "ddq_unpack_argmax": (ctypes.c_int, [_vp, _c_int64, _vp, _vp]),
+    "ddq_plan_step": (ctypes.c_int, [_vp, _vp, _vp, _c_int64, _c_int64, _vp, _c_int64, _vp,
+                                     _c_int64, _c_int64, _vp, _vp, _vp, _vp, _vp, _vp, _c_int64,
+                                     _c_int64, _vp]),
+    "ddq_paged_rope_kv": (ctypes.c_int, [_vp, _c_int64, _cache_p, _vp, _vp, _c_int64, _vp, _vp,
+                                         _vp, _c_int64, _c_int64, _vp]),
+    "ddq_paged_prefill_attention_workspace_size": (ctypes.c_size_t, [_c_int64] * 8),
+    "ddq_paged_decode_attention_workspace_size": (ctypes.c_size_t, [_c_int64] * 7),
+    "ddq_paged_prefill_attention": (ctypes.c_int, [_vp, _c_int64, _c_int64, _cache_p, _vp,
+                                                   _c_int64, _c_int64, _vp, _vp, _vp, _vp,
+                                                   _c_int64, _vp, ctypes.c_float, ctypes.c_float,
+                                                   _vp, _c_int64, _c_int64, _c_int64, _c_int64,
+                                                   _c_int64, _vp, ctypes.c_size_t, _vp]),
+    "ddq_paged_decode_attention": (ctypes.c_int, [_vp, _c_int64, _c_int64, _cache_p, _vp,
+                                                  _c_int64, _c_int64, _vp, _vp, _c_int64, _vp,
+                                                  ctypes.c_float, ctypes.c_float, _vp, _c_int64,
+                                                  _c_int64, _c_int64, _c_int64, _vp,
+                                                  ctypes.c_size_t, _vp]),
     "ddq_device_error": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int), _vp]),
     "ddq_set_debug": (ctypes.c_int, [ctypes.c_int, ctypes.c_uint64]),
     "ddq_read_trace": (ctypes.c_int, [_vp, ctypes.c_int, _vp]),
@@ -60,7 +87,7 @@ _SIGNATURES = {
 
 EXPORTED = tuple(_SIGNATURES)
 
-DTYPE_NONE, DTYPE_F16, DTYPE_F32 = 0, 1, 2
+DTYPE_NONE, DTYPE_F16, DTYPE_F32, DTYPE_BF16 = 0, 1, 2, 3
 ERR_SHAPE = 2  # DDQ_ERR_SHAPE: the entry does not take this shape
 
 _lock = threading.Lock()

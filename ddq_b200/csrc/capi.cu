@@ -140,6 +140,7 @@ extern "C" const char* ddq_status_string(int status) {
     case DDQ_ERR_DEVICE: return "no usable sm_100 device";
     case DDQ_ERR_LAUNCH: return "CUDA kernel launch failed";
     case DDQ_ERR_TIMEOUT: return "device-side bounded wait timed out";
+    case DDQ_ERR_PAGE: return "page, slot, length or position outside the paged cache";
     default: return "unknown ddq status";
   }
 }

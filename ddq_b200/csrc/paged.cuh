@@ -1,0 +1,95 @@
+// paged.cuh - what the paged KV-cache kernels share: the cache description,
+// the arguments of the attention kernels and the element types.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace ddq {
+
+// One pool of pages: k and v [num_pages, Hkv, page, D] through element strides
+// (D contiguous), pages of 2^page_shift rows.
+struct PgCache {
+  void* k;
+  void* v;
+  int64_t page_stride, head_stride, row_stride;
+  int num_pages, page_shift;
+  int Hkv, D;
+};
+
+struct PgAttnArgs {
+  PgCache c;
+  const void* q;            // [T, Hq, D], element strides
+  int64_t q_ts, q_hs;
+  void* out;                // [T, Hq, D]
+  int64_t o_ts, o_hs;
+  const int* table;         // [R, width], row stride table_stride
+  int64_t table_stride;
+  int width;
+  const int* lens;          // [R] keys of each request in its own pages
+  const int* cu;            // [R + 1] first query row of each request; null: one row each
+  const int* bidir;         // [R] or null: own keys every row of the request may attend
+  const int* prefix_pages;  // shared prefix (its rows come before the own ones) or null
+  int prefix_len;
+  const float* slopes;      // [Hq] or null
+  float scale, cap;
+  int T, R, Hq;
+};
+
+template <typename T>
+struct PgType;
+template <>
+struct PgType<__half> {
+  static __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+  static __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
+  static __device__ __forceinline__ float2 to_f2(uint32_t u) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct PgType<__nv_bfloat16> {
+  static __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+  static __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
+  static __device__ __forceinline__ float2 to_f2(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+// Keys of request r in its own pages: the length, never more than its table
+// row holds (a longer one is an error of the caller's, recorded).
+__device__ __forceinline__ int pg_len(const PgAttnArgs& a, int r) {
+  const int n = a.lens[r] < 0 ? 0 : a.lens[r];
+  const int64_t hold = (int64_t)a.width << a.c.page_shift;
+  if (n <= hold) return n;
+  record_device_error(DDQ_ERR_PAGE);
+  return (int)hold;
+}
+
+// A page number as the tables hold it, -1 (recorded) for one outside the pool.
+__device__ __forceinline__ int pg_check(const PgCache& c, int page) {
+  if ((unsigned)page < (unsigned)c.num_pages) return page;
+  record_device_error(DDQ_ERR_PAGE);
+  return -1;
+}
+
+int launch_plan_step(const int* cached, const int* fresh, int* table, int64_t table_stride,
+                     int width, const int* free_pages, int num_free, const int* free_head,
+                     int page_shift, int64_t prefix_len, int* cu, int* lens, int64_t* slots,
+                     int64_t* positions, int* seq_ids, int* free_head_out, int R, int T,
+                     cudaStream_t s);
+int launch_paged_rope_kv(const void* qkv, int64_t qkv_stride, const PgCache& c, bool bf16,
+                         const float* cos, const float* sin, int64_t max_pos,
+                         const int64_t* slots, const int64_t* positions, void* q_out, int64_t T,
+                         int Hq, cudaStream_t s);
+int launch_paged_attention(const PgAttnArgs& a, bool bf16, cudaStream_t s);
+
+}  // namespace ddq

@@ -45,14 +45,17 @@ typedef enum ddq_status {
   DDQ_ERR_WORKSPACE = 4,        /* workspace missing or smaller than required */
   DDQ_ERR_DEVICE = 5,           /* no sm_100 device / attribute query failed */
   DDQ_ERR_LAUNCH = 6,           /* CUDA launch error (cudaGetLastError) */
-  DDQ_ERR_TIMEOUT = 7           /* a device-side bounded wait gave up */
+  DDQ_ERR_TIMEOUT = 7,          /* a device-side bounded wait gave up */
+  DDQ_ERR_PAGE = 8              /* device error word: a page number, slot, length or position
+                                 * outside the cache, its table or the rotary rows */
 } ddq_status;
 
-/* Element type codes for bias / weight inputs. */
+/* Element type codes for bias / weight inputs and the paged cache. */
 enum {
   DDQ_DTYPE_NONE = 0,
   DDQ_DTYPE_F16 = 1,
-  DDQ_DTYPE_F32 = 2
+  DDQ_DTYPE_F32 = 2,
+  DDQ_DTYPE_BF16 = 3 /* paged operators only */
 };
 
 /* Human-readable text of a status code (static storage). */
@@ -359,8 +362,134 @@ int ddq_unpack_argmax(const uint64_t* packed, int64_t M, int64_t* ids,
                       void* stream);
 
 /*
+ * ---------------------------------------------------------------------------
+ * Paged KV cache: requests of different lengths in one pool of pages.  No
+ * reference counterpart as a whole; each operator names the part of the
+ * reference's dense-cache path that it takes the place of.
+ * ---------------------------------------------------------------------------
+ *
+ * A pool of num_pages pages of page_size rows (16, 32, 64, 128 or 256) for Hkv
+ * key/value heads of D = 64 or 128 dimensions, fp16 or bf16.  Element
+ * [page, g, row, d] of k and of v lies at page * page_stride + g * head_stride
+ * + row * row_stride + d (strides in elements, multiples of 8; k and v 16-byte
+ * aligned).  A table row lists a request's pages in order; entries past its
+ * length are not read.  A page number, slot or position outside the pool (or
+ * the rotary rows) is never followed: the write is left out, the attention of
+ * that request (and of no other) is unspecified, and the device error word is
+ * set to DDQ_ERR_PAGE.
+ */
+typedef struct ddq_paged_cache {
+  void* k;
+  void* v;
+  int64_t num_pages, page_size, Hkv, D;
+  int64_t page_stride, head_stride, row_stride;
+  int dtype; /* DDQ_DTYPE_F16 or DDQ_DTYPE_BF16 */
+} ddq_paged_cache;
+
+/*
+ * The plan of one step from the request lengths, on the device: which pages
+ * each request takes from the free list, and where each new token goes.
+ * Takes the place of the reference's single running length (engine.py:126-130).
+ *   cached, new_tokens  int32 [R]: tokens in the cache, tokens of this step
+ *                       (a negative length counts as 0; cached + new < 2^31 - 256)
+ *   block_table  int32 [R, table_width], row stride table_stride: the pages of
+ *                the cached tokens; the entries ceil(cached / page_size) ..
+ *                ceil((cached + new) / page_size) - 1 are written
+ *   free_pages   int32 [num_free]; free_head int32 [1] or NULL (0): the first
+ *                one not handed out yet
+ *   cu_new [R + 1]    exclusive sums of new_tokens
+ *   lens [R]          cached + new_tokens
+ *   slots [T]         int64 page * page_size + row, -1 for a token without a
+ *                     page (list exhausted, table full) and behind the last token
+ *   positions [T]     int64 prefix_len + index in the request; 0 behind the last
+ *   seq_ids [T]       int32 request of the token; -1 behind the last
+ *   free_head_out [1] free_head + pages taken (beyond num_free: that many are
+ *                     missing); not the same memory as free_head
+ * T is the number of token rows of the step (a capacity: sum(new_tokens) <= T
+ * is the caller's to keep; tokens past T are not written).  1 <= R <= 8192.
+ */
+int ddq_plan_step(const int32_t* cached, const int32_t* new_tokens, int32_t* block_table,
+                  int64_t table_stride, int64_t table_width, const int32_t* free_pages,
+                  int64_t num_free, const int32_t* free_head, int64_t page_size,
+                  int64_t prefix_len, int32_t* cu_new, int32_t* lens, int64_t* slots,
+                  int64_t* positions, int32_t* seq_ids, int32_t* free_head_out, int64_t R,
+                  int64_t T, void* stream);
+
+/*
+ * Rotary embedding of q and k and the write of k and v into their pages.
+ * Takes the place of the RoPE kernel (RoPe_d.cu:12-68, engine.py:219-220) and
+ * the cache write (engine.py:126-130, 222) for tokens of any requests.
+ *   qkv    [T, (Hq + 2 Hkv) * D] of the cache's type, row stride qkv_stride
+ *          (elements, multiple of 8)
+ *   cos, sin  fp32 [max_pos, D]; positions int64 [T], slots int64 [T] (< 0: the
+ *          row's k and v are not written; no slot twice)
+ *   q_out  [T, Hq, D]: rope(q) of every row
+ */
+int ddq_paged_rope_kv(const void* qkv, int64_t qkv_stride, const ddq_paged_cache* cache,
+                      const float* cos, const float* sin, int64_t max_pos, const int64_t* slots,
+                      const int64_t* positions, void* q_out, int64_t T, int64_t Hq,
+                      void* stream);
+
+/*
+ * Bytes of workspace of the two attention calls below (16-byte aligned, need
+ * not be filled; the partial results of a split key axis).
+ */
+size_t ddq_paged_prefill_attention_workspace_size(int64_t T, int64_t R, int64_t Hq, int64_t Hkv,
+                                                  int64_t D, int64_t table_width,
+                                                  int64_t page_size, int64_t prefix_len);
+size_t ddq_paged_decode_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                                 int64_t table_width, int64_t page_size,
+                                                 int64_t prefix_len);
+
+/*
+ * Attention of the new tokens of R requests, packed one after another, over
+ * their pages (which hold the new tokens' keys and values already).  Takes the
+ * place of the prompt attention of engine.py:225-251.
+ *   q, out  [T, Hq, D] of the cache's type, token and head strides in elements
+ *           (multiples of 8, 16-byte aligned)
+ *   cu_new  int32 [R + 1]: rows cu_new[r] .. cu_new[r + 1] - 1 are request r's
+ *           (its last ones); rows behind cu_new[R] are left as they are
+ *   lens    int32 [R]: keys of the request, its new tokens included
+ *   bidir   int32 [R] or NULL; slopes fp32 [Hq] or NULL; softcap 0: none
+ *   prefix_pages  int32 [ceil(prefix_len / page_size)] or NULL: prefix_len keys
+ *           in front of every request's own (stored once; it may end inside a page)
+ * Row i of n, at position p = prefix_len + len - n + i, attends the keys j of
+ * the prefix and of its request with j < max(p + 1, prefix_len + min(bidir,
+ * len)), score softcap * tanh(scale q.k / softcap) - slope |p - j|, softmax in
+ * fp32; a row without keys is zero.  The keys and values of a request must be
+ * finite; what lies behind them is not looked at.
+ */
+int ddq_paged_prefill_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                const ddq_paged_cache* cache, const int32_t* block_table,
+                                int64_t table_stride, int64_t table_width, const int32_t* cu_new,
+                                const int32_t* lens, const int32_t* bidir,
+                                const int32_t* prefix_pages, int64_t prefix_len,
+                                const float* slopes, float scale, float softcap, void* out,
+                                int64_t out_token_stride, int64_t out_head_stride, int64_t T,
+                                int64_t R, int64_t Hq, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+/*
+ * Decode attention, one token for each of B sequences: over prefix_len keys
+ * that all share (prefix_pages int32 [ceil(prefix_len / page_size)]), then the
+ * sequence's own lens[b] keys in its own pages.  Takes the place of the
+ * attention of a decode step (engine.py:225-251).  The query stands at position
+ * prefix_len + lens[b] - 1; scores, mask and types as above.  prefix_pages may
+ * be NULL with prefix_len 0.  A sequence without keys gives zeros.
+ */
+int ddq_paged_decode_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                               const ddq_paged_cache* cache, const int32_t* block_table,
+                               int64_t table_stride, int64_t table_width, const int32_t* lens,
+                               const int32_t* prefix_pages, int64_t prefix_len,
+                               const float* slopes, float scale, float softcap, void* out,
+                               int64_t out_token_stride, int64_t out_head_stride, int64_t B,
+                               int64_t Hq, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/*
  * Read (and clear) the device error word that bounded device-side waits set
- * when they give up.  Synchronises `stream`.  *code = 0 means no error.
+ * when they give up and the paged operators when they leave out a bad page.
+ * Synchronises `stream`.  *code = 0 means no error.
  */
 int ddq_device_error(int* code, void* stream);
 
