@@ -58,7 +58,7 @@ int check_attn(const void* q, int64_t q_ts, int64_t q_hs, const void* out, int64
   if (!q || !out || !table || !lens) return DDQ_ERR_INVALID_ARGUMENT;
   if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.f)
     return DDQ_ERR_INVALID_ARGUMENT;
-  if (Hq < 1 || Hq > 1024 || Hq % Hkv != 0 || T > kIntMax || table_width < 1 ||
+  if (T > kIntMax || Hq < 1 || Hq > 1024 || Hq % Hkv != 0 || T * Hq > kIntMax || table_width < 1 ||
       table_width > kIntMax || table_stride < table_width || q_ts < 0 || o_ts < 0 || q_hs < 0 ||
       o_hs < 0)
     return DDQ_ERR_SHAPE;
@@ -118,14 +118,36 @@ extern "C" int ddq_paged_rope_kv(const void* qkv, int64_t qkv_stride,
                               reinterpret_cast<cudaStream_t>(stream));
 }
 
+namespace {
+int sm_count() {
+  const int n = device_sm_count(current_device());
+  return n > 0 ? n : 148;
+}
+// o [count][rows][D] and lse [count][rows], fp32
+size_t parts_bytes(int64_t rows, int64_t D, int count) {
+  return count > 1 ? (size_t)count * rows * (D + 1) * sizeof(float) : 0;
+}
+PgParts make_parts(void* ws, int64_t rows, int64_t D, int count) {
+  if (count <= 1) return PgParts{nullptr, nullptr, rows, 0, 1};
+  float* o = static_cast<float*>(ws);
+  return PgParts{o, o + (size_t)count * rows * D, rows, 0, count};
+}
+bool prefill_shape(int64_t T, int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
+                   int64_t page_size, int64_t prefix_len) {
+  return T > 0 && R > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && D > 0 && table_width > 0 &&
+         page_size > 0 && prefix_len >= 0;
+}
+}  // namespace
+
 extern "C" size_t ddq_paged_prefill_attention_workspace_size(int64_t T, int64_t R, int64_t Hq,
                                                              int64_t Hkv, int64_t D,
                                                              int64_t table_width,
                                                              int64_t page_size,
                                                              int64_t prefix_len) {
-  (void)T, (void)R, (void)Hq, (void)Hkv, (void)D, (void)table_width, (void)page_size;
-  (void)prefix_len;
-  return 0;
+  if (!prefill_shape(T, R, Hq, Hkv, D, table_width, page_size, prefix_len)) return 0;
+  const int s = tc_splits(T, R, (int)Hq, (int)Hkv, prefix_len + table_width * page_size, true,
+                          sm_count());
+  return parts_bytes(T * Hq, D, s);
 }
 
 extern "C" size_t ddq_paged_decode_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv,
@@ -154,12 +176,20 @@ extern "C" int ddq_paged_prefill_attention(
                   block_table, table_stride, table_width, lens, scale, softcap, T, Hq, c.Hkv,
                   c.D);
   if (st) return st;
-  (void)workspace, (void)workspace_bytes;
+  const bool bf16 = cache->dtype == DDQ_DTYPE_BF16;
+  const int splits = tc_splits(T, R, (int)Hq, c.Hkv,
+                               prefix_len + (table_width << c.page_shift), true, sm_count());
+  if (splits > 1 && (!workspace || workspace_bytes < parts_bytes(T * Hq, c.D, splits)))
+    return DDQ_ERR_WORKSPACE;
+  if (splits > 1 && !aligned16(workspace)) return DDQ_ERR_ALIGNMENT;
+  const PgParts parts = make_parts(workspace, T * Hq, c.D, splits);
   PgAttnArgs a{c, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
                block_table, table_stride, (int)table_width, lens, cu_new, bidir, prefix_pages,
                (int)prefix_len, slopes, scale, softcap, (int)T, (int)R, (int)Hq};
-  return launch_paged_attention(a, cache->dtype == DDQ_DTYPE_BF16,
-                                reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  st = launch_paged_tc(a, bf16, parts, splits, wait_timeout_ns(), s);
+  if (st || splits == 1) return st;
+  return launch_paged_merge(a, bf16, parts, s);
 }
 
 extern "C" int ddq_paged_decode_attention(

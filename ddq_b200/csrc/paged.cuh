@@ -37,6 +37,17 @@ struct PgAttnArgs {
   int T, R, Hq;
 };
 
+// Parts of a split key axis: part z of row t * Hq + h holds the row's output
+// over its keys, o[z][row][D], and log2 of the sum of its weights, lse[z][row]
+// (-inf: no keys, o not written).  A kernel writes from part `first` on; o null:
+// one part, written to the output itself.
+struct PgParts {
+  float* o;
+  float* lse;
+  int64_t rows;
+  int first, count;
+};
+
 template <typename T>
 struct PgType;
 template <>
@@ -90,6 +101,10 @@ int launch_paged_rope_kv(const void* qkv, int64_t qkv_stride, const PgCache& c, 
                          const float* cos, const float* sin, int64_t max_pos,
                          const int64_t* slots, const int64_t* positions, void* q_out, int64_t T,
                          int Hq, cudaStream_t s);
+int tc_splits(int64_t T, int64_t R, int Hq, int Hkv, int64_t keys, bool ragged, int sms);
+int launch_paged_tc(const PgAttnArgs& a, bool bf16, const PgParts& parts, int splits,
+                    unsigned long long tmo, cudaStream_t s);
+int launch_paged_merge(const PgAttnArgs& a, bool bf16, const PgParts& parts, cudaStream_t s);
 int launch_paged_attention(const PgAttnArgs& a, bool bf16, cudaStream_t s);
 
 }  // namespace ddq

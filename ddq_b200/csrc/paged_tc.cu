@@ -1,0 +1,623 @@
+// paged_tc.cu - paged attention of many query rows on the tcgen05 tensor cores:
+// the new tokens of ragged requests, and the rows of a decode batch over the
+// prefix that they share.  The mathematics is in paged_attn.cu.
+//
+// The G = Hq / Hkv query heads of a key/value head are packed with the tokens:
+// row rr of a request is token rr / G, head g G + rr % G, so that a tile of 256
+// rows covers 256 / G consecutive tokens, every key tile is used by all heads
+// that share it, and few tokens still fill a tile (a decode batch of B rows is
+// a request of B tokens).
+//
+// One CTA per (tile, key/value head, split of the key axis), two 128-row
+// halves, one key tile of 128 at a time:
+//   S_t = Q_t K^T   tcgen05.mma, 128 x 128, from shared memory into TMEM
+//   P_t = exp2(x - m) of the scores x in log2 units, one thread per row, fp32;
+//         rounded once to the operand type (weights reach PV in 11 or 8 bits,
+//         the sum l is of the unrounded ones) and put back into TMEM
+//   O_t += P_t V    tcgen05.mma, A from TMEM, V from shared memory as it lies
+//         (keys in rows: an MN-major B operand, no transpose)
+// The running maximum only moves when a tile exceeds it by more than 8 (a
+// factor 256, harmless in fp32 and in the type of P), so O in TMEM is rarely
+// rescaled: after the first tiles a row's maximum hardly grows.
+//
+// Warps 0-3 and 4-7: softmax of half 0 and 1.  Warp 8: TMA, one box per page
+// and 64 dimensions, each lane its own.  Warp 9: MMA issue.  While one half is
+// in its softmax the tensor core works for the other.  64-wide heads leave TMEM
+// for P beside S, so S of the next tile is made during the softmax of this one;
+// with 128-wide heads P takes S's place and it follows PV.
+#include <cudaTypedefs.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "launch.cuh"
+#include "paged.cuh"
+#include "sm100_ptx.cuh"
+
+namespace ddq {
+
+constexpr int TC_KV = 128;       // keys per tile
+constexpr int TC_HALF = 128;     // rows per half
+constexpr int TC_ROWS = 256;     // rows per CTA
+constexpr int TC_NT = 384;        // two softmax warpgroups and one for TMA and MMA issue
+// Registers a thread: launched with 168 (3 warps on each quarter of the SM);
+// the third warpgroup gives up 80, the softmax ones take 40 each: 256 x 208 +
+// 128 x 88 = 384 x 168.  A softmax thread holds its row of 128 scores.
+constexpr int TC_REG_SOFTMAX = 208, TC_REG_ISSUE = 88;
+constexpr float TC_LAZY = 8.f;   // log2 units
+
+template <int D>
+struct TcLayout {
+  static constexpr int HB = TC_KV * 128;         // bytes of 128 rows x 64 elements
+  static constexpr int TILE = (D / 64) * HB;     // one K or V tile, one half of Q
+  static constexpr int ST = D == 64 ? 8 : 4;     // ring stages (K and V alternate)
+  static constexpr int OFF_RING = 2 * TILE;
+  static constexpr int OFF_BAR = OFF_RING + ST * TILE;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;
+  static constexpr bool SEP = D == 64;           // P beside S
+  static constexpr int COL_S = 0, COL_P = SEP ? 256 : 0, STEP_P = SEP ? 64 : 128;
+  static constexpr int COL_O = SEP ? 384 : 256;
+};
+
+__device__ __forceinline__ float tc_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float tc_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void tc_regs(uint32_t* r) {  // the loads above are complete
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile(""
+                 : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]),
+                   "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+
+// mbar_wait with one answer for the warp: the TMEM loads and stores after it
+// need all lanes, also when a wait gives up.
+__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, uint64_t tmo,
+                                        volatile int* abort) {
+  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, tmo, abort));
+}
+
+template <typename E, int D>
+__global__ void __launch_bounds__(TC_NT, 1)
+    paged_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
+                    const __grid_constant__ CUtensorMap tm_v, const PgAttnArgs a,
+                    const PgParts parts, const int splits, const unsigned long long tmo) {
+  using L = TcLayout<D>;
+  using Ty = PgType<E>;
+  constexpr bool SEP = L::SEP;
+  extern __shared__ uint8_t tc_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const uint32_t sbase = ptx::smem_u32(smem);
+  __shared__ int found[2], wsum[TC_NT / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = a.Hq / a.c.Hkv, g = blockIdx.y, z = blockIdx.z;
+
+  const uint32_t bar_full = sbase + L::OFF_BAR;
+  const uint32_t bar_empty = bar_full + 8 * L::ST;
+  const uint32_t bar_q = bar_empty + 8 * L::ST;
+  const uint32_t bar_s = bar_q + 8;         // [2] scores ready
+  const uint32_t bar_sfree = bar_s + 16;    // [2] scores read (SEP)
+  const uint32_t bar_p = bar_sfree + 16;    // [2] weights ready
+  const uint32_t bar_pv = bar_p + 16;       // [2] PV done
+  const uint32_t bar_drain = bar_pv + 16;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_BAR + 8 * (2 * L::ST + 10));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  if (tid == 0) {
+    for (int s = 0; s < L::ST; ++s) {
+      ptx::mbar_init(bar_full + 8 * s, 1);
+      ptx::mbar_init(bar_empty + 8 * s, 1);
+    }
+    ptx::mbar_init(bar_q, TC_ROWS);
+    for (int t = 0; t < 2; ++t) {
+      ptx::mbar_init(bar_s + 8 * t, 1);
+      ptx::mbar_init(bar_sfree + 8 * t, TC_HALF);
+      ptx::mbar_init(bar_p + 8 * t, TC_HALF);
+      ptx::mbar_init(bar_pv + 8 * t, 1);
+    }
+    ptx::mbar_init(bar_drain, 1);
+    *abort_flag = 0;
+    found[0] = -1;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tm_k);
+    ptx::prefetch_tmap(&tm_v);
+  }
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
+  __syncthreads();
+
+  // ---- the request and the tile of this CTA
+  int r = 0, tile = blockIdx.x, t_first = 0, n = a.T;
+  if (a.cu) {
+    int run = 0;
+    for (int base = 0; base < a.R; base += TC_NT) {
+      const int rr = base + tid;
+      int c0 = 0, cn = 0;
+      if (rr < a.R) {
+        c0 = a.cu[rr];
+        cn = a.cu[rr + 1] - c0;
+        if (c0 < 0 || c0 >= a.T || cn < 0) cn = 0;
+        cn = min(cn, a.T - c0);
+      }
+      const int tiles = (cn * G + TC_ROWS - 1) / TC_ROWS;
+      int s = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += u;
+      }
+      if (lane == 31) wsum[warp] = s;
+      __syncthreads();
+      int before = run;
+      for (int w = 0; w < TC_NT / 32; ++w) {
+        const int x = wsum[w];
+        if (w < warp) before += x;
+        run += x;
+      }
+      s += before;
+      if (tile < s && tile >= s - tiles) {
+        found[0] = rr;
+        found[1] = tile - (s - tiles);
+      }
+      __syncthreads();
+      if (found[0] >= 0) break;
+    }
+    r = found[0];
+    if (r < 0) return;  // the grid covers the most tiles that T rows can make
+    tile = found[1];
+    t_first = a.cu[r];
+    n = min(a.cu[r + 1] - t_first, a.T - t_first);
+  }
+  const int P = a.prefix_len;
+  const int len = a.cu ? pg_len(a, r) : 0;
+  const int least = a.cu ? (a.bidir ? P + min(a.bidir[r], len) : 0) : P;
+  const int row0 = tile * TC_ROWS, nrow = min(TC_ROWS, n * G - row0);
+  const int halves = nrow > TC_HALF ? 2 : 1;
+  // keys of the row of token i: those below end(i); the last row has the most
+  auto end_of = [&](int i) {
+    const int e = a.cu ? P + len - n + i + 1 : 0;
+    return max(max(e, least), 0);
+  };
+  const int end_max = end_of((row0 + nrow - 1) / G);
+  const int np = (min(P, end_max) + TC_KV - 1) / TC_KV;
+  const int nt = np + (max(end_max - P, 0) + TC_KV - 1) / TC_KV;
+  const int lo = (int)((int64_t)nt * z / splits), cnt = (int)((int64_t)nt * (z + 1) / splits) - lo;
+  // tile k of this CTA: first key, keys that exist behind it, its list
+  auto key0 = [&](int k) { return lo + k < np ? (lo + k) * TC_KV : P + (lo + k - np) * TC_KV; };
+  auto limit = [&](int k) { return lo + k < np ? P : P + len; };
+
+  uint32_t tmem = 0;
+  if (cnt > 0) {  // uniform over the CTA
+    if (warp == 9) {
+      ptx::tmem_alloc(ptx::smem_u32(tmem_holder), 512);
+      ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    tmem = *tmem_holder;
+  }
+
+  if (warp < 8) {
+    if (cnt > 0) ptx::reg_inc<TC_REG_SOFTMAX>();
+    // ---------------------------------------------------------------- softmax
+    const int t = warp >> 2;
+    const int rr = row0 + tid;                  // tid < 256: both halves in order
+    const bool real = tid < nrow;
+    const int i = real ? rr / G : 0, h = g * G + (real ? rr % G : 0);
+    const int tok = t_first + i;
+    const int end = real ? end_of(i) : 0;
+    const int pos = a.cu ? P + len - n + i : P + pg_len(a, real ? tok : 0) - 1;
+    float m = -INFINITY, l = 0.f;
+    const bool half_on = t < halves;
+    bool ok = true;
+    if (cnt > 0) {
+      // this row of Q, K-major with the 128-byte swizzle
+      uint8_t* qs = smem + t * L::TILE + (tid & 127) * 128;
+      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const E*>(a.q) +
+                                                        tok * a.q_ts + (int64_t)h * a.q_hs);
+      uint4 v[D / 8];
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) v[c] = real ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c)
+        *reinterpret_cast<uint4*>(qs + (c >> 3) * L::HB + (((c & 7) ^ (tid & 7)) << 4)) = v[c];
+      ptx::fence_proxy_async_smem();
+      ptx::mbar_arrive(bar_q);
+    }
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + L::COL_S + t * 128 + lanes;
+    const uint32_t tp = tmem + L::COL_P + t * L::STEP_P + lanes;
+    const uint32_t to = tmem + L::COL_O + t * D + lanes;
+    if (half_on && cnt > 0) {
+      constexpr float LOG2E = 1.4426950408889634f;
+      const bool plain = a.cap == 0.f && a.slopes == nullptr && a.scale > 0.f;
+      const float mul = plain ? a.scale * LOG2E : 1.f;
+      const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.f;
+      for (int k = 0; k < cnt; ++k) {
+        const int j0 = key0(k);
+        ok = tc_wait(bar_s + 8 * t, (uint32_t)k & 1u, tmo, abort_flag);
+        // (P in S's place: the PV of the tile before is done too, as its MMAs
+        // were issued before those of S; its barrier is waited for here so that
+        // no phase of it is skipped)
+        if (!SEP && ok && k > 0)
+          ok = tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        uint32_t u[128];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) ptx::tmem_ld_32x32b_x32(ts + c, u + c);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tc_regs(u + c);
+        if constexpr (SEP) {
+          ptx::tc_fence_before();
+          ptx::mbar_arrive(bar_sfree + 8 * t);
+        }
+        float* s = reinterpret_cast<float*>(u);
+        if (!plain) {  // to log2 units, capped and biased
+          if (a.cap > 0.f) {
+            // cap tanh(y / cap) = cap - 2 cap / (exp(2 y / cap) + 1): an absolute
+            // error of a few 2^-23 cap, also where the exponential overflows
+            const float kk = 2.f * LOG2E * a.scale / a.cap, A = a.cap * LOG2E;
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+              s[c] = fmaf(-2.f * A, tc_rcp(tc_exp2(s[c] * kk) + 1.f), A);
+          } else {
+            const float kk = a.scale * LOG2E;
+#pragma unroll
+            for (int c = 0; c < 128; ++c) s[c] *= kk;
+          }
+          if (a.slopes) {
+            const float d0 = (float)(pos - j0);
+#pragma unroll
+            for (int c = 0; c < 128; ++c) s[c] = fmaf(-slope, fabsf(d0 - (float)c), s[c]);
+          }
+        }
+        const int lim = min(end, limit(k)) - j0;  // keys of this tile that the row attends
+        if (!__all_sync(0xffffffffu, lim >= TC_KV)) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c >= lim) s[c] = -INFINITY;
+        }
+        float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
+#pragma unroll
+        for (int c = 4; c < 128; c += 4) {
+          x0 = fmaxf(x0, s[c]);
+          x1 = fmaxf(x1, s[c + 1]);
+          x2 = fmaxf(x2, s[c + 2]);
+          x3 = fmaxf(x3, s[c + 3]);
+        }
+        const float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * mul;
+        float alpha = 1.f;
+        if (mx > m + TC_LAZY) {  // also the first keys of the row (m = -inf)
+          if (m != -INFINITY) alpha = tc_exp2(m - mx);
+          m = mx;
+          l *= alpha;
+        }
+        if (k > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          if constexpr (SEP) {
+            ok = tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
+            if (!ok) break;
+            ptx::tc_fence_after();
+          }
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            ptx::tmem_ld_32x32b_x32(to + c, o);
+            ptx::tmem_ld_wait();
+            tc_regs(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            ptx::tmem_st_32x32b_x32(to + c, o);
+          }
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int c = 0; c < 128; c += 2) {
+          const float p0 = tc_exp2(fmaf(s[c], mul, -mu)), p1 = tc_exp2(fmaf(s[c + 1], mul, -mu));
+          l0 += p0;
+          l1 += p1;
+          u[c >> 1] = Ty::pack(p0, p1);
+        }
+        l += l0 + l1;
+        if (SEP && k > 0) {  // P of the tile before has been read
+          ok = tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
+          if (!ok) break;
+          ptx::tc_fence_after();
+        }
+        ptx::tmem_st_32x32b_x32(tp, u);
+        ptx::tmem_st_32x32b_x32(tp + 32, u + 32);
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(bar_p + 8 * t);
+      }
+      if (ok) ok = tc_wait(bar_pv + 8 * t, (uint32_t)(cnt - 1) & 1u, tmo, abort_flag);
+      ptx::tc_fence_after();
+    }
+    // ---- O / l, or the split's part of it.  Every lane takes part in the TMEM
+    // loads; a half without rows, and a row behind the last, stores nothing.
+    if (half_on && ok) {
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: 0; NaN stays
+      E* dst = reinterpret_cast<E*>(a.out) + tok * a.o_ts + (int64_t)h * a.o_hs;
+      const int64_t prow = (int64_t)tok * a.Hq + h;
+      float* po = parts.o ? parts.o + ((int64_t)(parts.first + z) * parts.rows + prow) * D : nullptr;
+      if (parts.o && real)
+        parts.lse[(int64_t)(parts.first + z) * parts.rows + prow] =
+            l == 0.f ? -INFINITY : m + log2f(l);
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (cnt > 0) {
+          ptx::tmem_ld_32x32b_x32(to + c, o);
+          ptx::tmem_ld_wait();
+          tc_regs(o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        float* f = reinterpret_cast<float*>(o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = l == 0.f ? 0.f : f[e] * inv;
+        if (real && po) {
+          if (l != 0.f) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(po + c + e) =
+                  make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+          }
+        } else if (real) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8)
+            *reinterpret_cast<uint4*>(dst + c + e) =
+                make_uint4(Ty::pack(f[e], f[e + 1]), Ty::pack(f[e + 2], f[e + 3]),
+                           Ty::pack(f[e + 4], f[e + 5]), Ty::pack(f[e + 6], f[e + 7]));
+        }
+      }
+    }
+  } else if (cnt > 0) {
+    ptx::reg_dec<TC_REG_ISSUE>();
+    if (warp == 8) {
+    // -------------------------------------------------------------------- TMA
+    const int br = min(1 << a.c.page_shift, TC_KV);   // rows of a box
+    const int nb = TC_KV / br;                        // boxes per tile and 64 dimensions
+    const int box = lane % nb, dh = lane / nb;        // this lane's
+    const int* own = a.table + (int64_t)r * a.table_stride;
+    int g_ring = 0;
+    bool ok = true;
+    for (int k = 0; k < cnt && ok; ++k) {
+      const bool shared = lo + k < np;
+      const int off = (shared ? (lo + k) : (lo + k - np)) * TC_KV + box * br;  // in its list
+      const int have = limit(k) - key0(k);
+      bool mine = dh < D / 64 && box * br < have;
+      int page = 0;
+      if (mine) {
+        page = pg_check(a.c, (shared ? a.prefix_pages : own)[off >> a.c.page_shift]);
+        mine = page >= 0;
+      }
+      const int prow = off & ((1 << a.c.page_shift) - 1);
+      const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, mine)) * br * 128u;
+#pragma unroll
+      for (int kv = 0; kv < 2 && ok; ++kv, ++g_ring) {
+        const int s = g_ring % L::ST;
+        ok = tc_wait(bar_empty + 8 * s, ((uint32_t)(g_ring / L::ST) & 1u) ^ 1u, tmo,
+                            abort_flag);
+        if (!ok) break;
+        if (lane == 0) ptx::mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
+        __syncwarp();
+        if (mine)
+          ptx::tma_load_4d(sbase + L::OFF_RING + s * L::TILE + dh * L::HB + box * br * 128,
+                           kv ? &tm_v : &tm_k, dh * 64, prow, g, page, bar_full + 8 * s);
+      }
+    }
+    if (!ok) {  // copies in flight land before the shared memory goes
+      for (int q = g_ring > L::ST ? g_ring - L::ST : 0; q < g_ring; ++q) {
+        const long long t0 = clock64();
+        while (!ptx::mbar_try_wait(bar_full + 8 * (q % L::ST), (uint32_t)(q / L::ST) & 1u))
+          if (clock64() - t0 > (long long)(tmo * 2ull)) break;
+      }
+    }
+    } else if (warp == 9) {
+    // -------------------------------------------------------------------- MMA
+    constexpr bool BF = sizeof(E) == 2 && !std::is_same<E, __half>::value;
+    constexpr uint32_t id_qk = ptx::idesc_16_f32(TC_HALF, TC_KV, BF, false);
+    constexpr uint32_t id_pv = ptx::idesc_16_f32(TC_HALF, D, BF, true);
+    const uint64_t dq = ptx::smem_desc_sw128(sbase);
+    const uint64_t dk = ptx::smem_desc_sw128(sbase + L::OFF_RING);
+    const uint64_t dv = ptx::smem_desc_sw128_mn(sbase + L::OFF_RING, L::HB);
+    auto stage = [&](int k, int kv) { return (2 * k + kv) % L::ST; };
+    auto wait_full = [&](int k, int kv) {
+      return tc_wait(bar_full + 8 * stage(k, kv),
+                            (uint32_t)((2 * k + kv) / L::ST) & 1u, tmo, abort_flag);
+    };
+    auto qk = [&](int k, int t) {
+      if (lane == 0) {
+        const uint64_t b0 = dk + (uint64_t)((stage(k, 0) * L::TILE) >> 4);
+        const uint64_t a0 = dq + (uint64_t)((t * L::TILE) >> 4);
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) {
+          const uint64_t o = (uint64_t)(((e >> 2) * L::HB + (e & 3) * 32) >> 4);
+          ptx::mma_f16_ss(tmem + L::COL_S + t * 128, a0 + o, b0 + o, id_qk, e != 0 ? 1u : 0u);
+        }
+        ptx::mma_commit(bar_s + 8 * t);
+        if (t == halves - 1) ptx::mma_commit(bar_empty + 8 * stage(k, 0));
+      }
+      __syncwarp();
+    };
+    auto pv = [&](int k, int t) {
+      if (lane == 0) {
+        const uint64_t b0 = dv + (uint64_t)((stage(k, 1) * L::TILE) >> 4);
+        const uint32_t p0 = tmem + L::COL_P + t * L::STEP_P;
+#pragma unroll
+        for (int e = 0; e < TC_KV / 16; ++e)
+          ptx::mma_f16_ts(tmem + L::COL_O + t * D, p0 + e * 8, b0 + (uint64_t)((e * 2048) >> 4),
+                          id_pv, (k | e) != 0 ? 1u : 0u);
+        ptx::mma_commit(bar_pv + 8 * t);
+        if (t == halves - 1) ptx::mma_commit(bar_empty + 8 * stage(k, 1));
+      }
+      __syncwarp();
+    };
+    bool ok = tc_wait(bar_q, 0, tmo, abort_flag) && wait_full(0, 0);
+    ptx::tc_fence_after();
+    if (ok)
+      for (int t = 0; t < halves; ++t) qk(0, t);
+    for (int k = 0; k < cnt && ok; ++k) {
+      for (int t = 0; t < halves && ok; ++t) {
+        if (SEP && k + 1 < cnt) {
+          if (t == 0) ok = wait_full(k + 1, 0);
+          ok = ok && tc_wait(bar_sfree + 8 * t, (uint32_t)k & 1u, tmo, abort_flag);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          qk(k + 1, t);
+        }
+        if (t == 0) {
+          ok = wait_full(k, 1);
+          if (!ok) break;
+          const int have = limit(k) - key0(k);
+          if (have < TC_KV) {
+            // the rows behind the last key may hold anything (or were not
+            // loaded): their weights are zero, and 0 x NaN is NaN
+            uint8_t* vs = smem + L::OFF_RING + stage(k, 1) * L::TILE;
+            for (int x = have * 8 + lane; x < TC_KV * 8; x += 32)
+#pragma unroll
+              for (int hb = 0; hb < D / 64; ++hb)
+                *reinterpret_cast<uint4*>(vs + hb * L::HB + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        ok = tc_wait(bar_p + 8 * t, (uint32_t)k & 1u, tmo, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        pv(k, t);
+        if (!SEP && k + 1 < cnt) {
+          if (t == 0) ok = wait_full(k + 1, 0);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          qk(k + 1, t);
+        }
+      }
+    }
+    if (!ok) {
+      if (lane == 0) ptx::mma_commit(bar_drain);
+      const long long t0 = clock64();
+      while (!ptx::mbar_try_wait(bar_drain, 0))
+        if (clock64() - t0 > (long long)(tmo * 2ull)) break;
+    }
+    }
+  }
+  if (cnt > 0) {
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && *abort_flag) record_device_error(DDQ_ERR_TIMEOUT);
+    if (warp == 9) {
+      ptx::tc_fence_after();
+      ptx::tmem_dealloc(tmem, 512);
+    }
+  }
+}
+
+namespace {
+PFN_cuTensorMapEncodeTiled_v12000 tc_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+}  // namespace
+
+// The pool as {D, page, Hkv, pages} with boxes of 64 dimensions x `rows` rows.
+int pg_tensor_map(CUtensorMap* m, const PgCache& c, const void* base, bool bf16, int rows) {
+  auto enc = tc_encoder();
+  if (!enc) return DDQ_ERR_DEVICE;
+  cuuint64_t dims[4] = {(cuuint64_t)c.D, (cuuint64_t)1 << c.page_shift, (cuuint64_t)c.Hkv,
+                        (cuuint64_t)c.num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)c.row_stride * 2, (cuuint64_t)c.head_stride * 2,
+                           (cuuint64_t)c.page_stride * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r =
+      enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+          const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? DDQ_OK : DDQ_ERR_SHAPE;
+}
+
+// The most tiles that T rows of R requests make (a request ends inside a tile).
+int64_t tc_tiles(int64_t T, int64_t R, int64_t G, bool ragged) {
+  if (!ragged) return (T * G + TC_ROWS - 1) / TC_ROWS;
+  return T * G / TC_ROWS + (R < T ? R : T);
+}
+
+// Splits of the key axis: as many as give every SM a CTA, of at least two key
+// tiles each.
+int tc_splits(int64_t T, int64_t R, int Hq, int Hkv, int64_t keys, bool ragged, int sms) {
+  const int64_t ctas = tc_tiles(T, R, Hq / Hkv, ragged) * Hkv;
+  int64_t s = sms / ctas;
+  const int64_t most = (keys + 2 * TC_KV - 1) / (2 * TC_KV);
+  s = s > most ? most : s;
+  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+int launch_paged_tc(const PgAttnArgs& a, bool bf16, const PgParts& parts, int splits,
+                    unsigned long long tmo, cudaStream_t s) {
+  const int G = a.Hq / a.c.Hkv;
+  const int64_t tiles = tc_tiles(a.T, a.R, G, a.cu != nullptr);
+  if (tiles > 0x7fffffff || a.c.Hkv > 65535) return DDQ_ERR_SHAPE;
+  CUtensorMap tk, tv;
+  const int br = (1 << a.c.page_shift) < TC_KV ? (1 << a.c.page_shift) : TC_KV;
+  int st = pg_tensor_map(&tk, a.c, a.c.k, bf16, br);
+  if (!st) st = pg_tensor_map(&tv, a.c, a.c.v, bf16, br);
+  if (st) return st;
+  const int dev = current_device();
+  static SmemAttrOnce attr[2][2];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)tiles, (unsigned)a.c.Hkv, (unsigned)splits);
+  cfg.blockDim = dim3(TC_NT);
+  cfg.stream = s;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaSuccess;
+  auto go = [&](auto kern, SmemAttrOnce& once, int smem) -> int {
+    const int ast = ensure_smem_attr(once, dev, kern, smem);
+    if (ast) return ast;
+    cfg.dynamicSmemBytes = smem;
+    e = cudaLaunchKernelEx(&cfg, kern, tk, tv, a, parts, splits, tmo);
+    return DDQ_OK;
+  };
+  if (a.c.D == 64)
+    st = bf16 ? go(paged_tc_kernel<__nv_bfloat16, 64>, attr[0][1], TcLayout<64>::SMEM)
+              : go(paged_tc_kernel<__half, 64>, attr[0][0], TcLayout<64>::SMEM);
+  else
+    st = bf16 ? go(paged_tc_kernel<__nv_bfloat16, 128>, attr[1][1], TcLayout<128>::SMEM)
+              : go(paged_tc_kernel<__half, 128>, attr[1][0], TcLayout<128>::SMEM);
+  if (st) return st;
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return DDQ_ERR_LAUNCH;
+  }
+  return check_launch();
+}
+
+}  // namespace ddq
