@@ -1,8 +1,8 @@
 """Build the native library ``ddq_b200/lib/libddq_b200.so`` in-tree.
 
 Every ``csrc/*.cu`` file is compiled for sm_100a only
-(``-gencode arch=compute_100a,code=sm_100a``) with relocatable device code,
-in parallel, then device-linked into one shared library that exports the C ABI
+(``-gencode arch=compute_100a,code=sm_100a``) with relocatable device code
+(but for WHOLE_PROGRAM), in parallel, then device-linked into one shared library that exports the C ABI
 declared in ``include/ddq_b200.h``.  The library links the CUDA runtime
 statically and does not depend on torch.  Sources are rebuilt only when a
 ``.cu``/``.cuh``/header file is newer than the library.
@@ -31,6 +31,10 @@ LIB_PATH = os.path.join(LIB_DIR, "libddq_b200.so")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-rdc=true", "-Xcompiler", "-fPIC",
               "-Xcompiler", "-O3", "--expt-relaxed-constexpr", "-I", INCLUDE]
+# compiled without relocatable device code: a kernel that moves registers
+# between its warpgroups (ptxas ignores that across compilation units).  Such a
+# file refers to no device symbol of another one.
+WHOLE_PROGRAM = ("paged_tc.cu",)
 
 
 def _nvcc() -> str:
@@ -58,7 +62,10 @@ def is_stale() -> bool:
 
 def _compile(src: str, verbose: bool) -> str:
     obj = os.path.join(BUILD_DIR, os.path.basename(src)[:-3] + ".o")
-    cmd = [_nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, "-c", src, "-o", obj]
+    flags = NVCC_FLAGS
+    if os.path.basename(src) in WHOLE_PROGRAM:
+        flags = [f for f in NVCC_FLAGS if f != "-rdc=true"] + ["-DDDQ_WHOLE_PROGRAM"]
+    cmd = [_nvcc(), *ARCH_FLAGS, *flags, "-c", src, "-o", obj]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
     r = subprocess.run(cmd, capture_output=True, text=True)

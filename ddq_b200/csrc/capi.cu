@@ -42,6 +42,22 @@ int check_launch() {
   return e == cudaSuccess ? DDQ_OK : DDQ_ERR_LAUNCH;
 }
 
+int* device_error_word() {
+  static std::once_flag once[kMaxDev];
+  static int* ptr[kMaxDev];
+  const int d = current_device();
+  if (d < 0 || d >= kMaxDev) return nullptr;
+  std::call_once(once[d], [d] {
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_device_error) != cudaSuccess) {
+      cudaGetLastError();
+      p = nullptr;
+    }
+    ptr[d] = static_cast<int*>(p);
+  });
+  return ptr[d];
+}
+
 namespace {
 // Kernel choice by M: M < tc_min_m -> CUDA-core skinny kernel; M <= 64 ->
 // decode kernel (e4m3 tensor cores, activation planes); M > 64 -> prefill

@@ -119,6 +119,7 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+#ifndef DDQ_WHOLE_PROGRAM  // a file of its own sees no device symbol of the others
 // Device error word set by bounded waits that give up (read by ddq_device_error).
 extern __device__ int g_device_error;
 
@@ -142,12 +143,15 @@ __device__ __forceinline__ void trace_stamp(bool on, int slot) {
   }
 }
 
+#endif  // DDQ_WHOLE_PROGRAM
+
 // ----------------------------------------------------------------------------
 // Host-side helpers
 // ----------------------------------------------------------------------------
 int device_sm_count(int device);
 int current_device();
 int check_launch();
+int* device_error_word();  // its address on the current device (null: no device)
 bool pdl_enabled();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -28,7 +28,7 @@ int check_cache(const ddq_paged_cache* c, PgCache* out) {
       c->head_stride % 8 != 0 || c->row_stride % 8 != 0)
     return DDQ_ERR_ALIGNMENT;
   *out = PgCache{c->k, c->v, c->page_stride, c->head_stride, c->row_stride,
-                 (int)c->num_pages, sh, (int)c->Hkv, (int)c->D};
+                 (int)c->num_pages, sh, (int)c->Hkv, (int)c->D, nullptr};
   return DDQ_OK;
 }
 
@@ -176,6 +176,7 @@ extern "C" int ddq_paged_prefill_attention(
                   block_table, table_stride, table_width, lens, scale, softcap, T, Hq, c.Hkv,
                   c.D);
   if (st) return st;
+  if (!(c.err = device_error_word())) return DDQ_ERR_DEVICE;
   const bool bf16 = cache->dtype == DDQ_DTYPE_BF16;
   const int splits = tc_splits(T, R, (int)Hq, c.Hkv,
                                prefix_len + (table_width << c.page_shift), true, sm_count());
@@ -209,6 +210,7 @@ extern "C" int ddq_paged_decode_attention(
                   c.D);
   if (st) return st;
   (void)workspace, (void)workspace_bytes;
+  if (!(c.err = device_error_word())) return DDQ_ERR_DEVICE;
   PgAttnArgs a{c, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
                block_table, table_stride, (int)table_width, lens, nullptr, nullptr, prefix_pages,
                (int)prefix_len, slopes, scale, softcap, (int)B, (int)B, (int)Hq};

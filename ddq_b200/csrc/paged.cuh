@@ -16,7 +16,10 @@ struct PgCache {
   int64_t page_stride, head_stride, row_stride;
   int num_pages, page_shift;
   int Hkv, D;
+  int* err;  // the device error word
 };
+
+__device__ __forceinline__ void pg_error(const PgCache& c, int code) { atomicCAS(c.err, 0, code); }
 
 struct PgAttnArgs {
   PgCache c;
@@ -81,14 +84,14 @@ __device__ __forceinline__ int pg_len(const PgAttnArgs& a, int r) {
   const int n = a.lens[r] < 0 ? 0 : a.lens[r];
   const int64_t hold = (int64_t)a.width << a.c.page_shift;
   if (n <= hold) return n;
-  record_device_error(DDQ_ERR_PAGE);
+  pg_error(a.c, DDQ_ERR_PAGE);
   return (int)hold;
 }
 
 // A page number as the tables hold it, -1 (recorded) for one outside the pool.
 __device__ __forceinline__ int pg_check(const PgCache& c, int page) {
   if ((unsigned)page < (unsigned)c.num_pages) return page;
-  record_device_error(DDQ_ERR_PAGE);
+  pg_error(c, DDQ_ERR_PAGE);
   return -1;
 }
 

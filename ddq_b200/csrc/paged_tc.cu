@@ -195,20 +195,32 @@ __global__ void __launch_bounds__(TC_NT, 1)
   auto key0 = [&](int k) { return lo + k < np ? (lo + k) * TC_KV : P + (lo + k - np) * TC_KV; };
   auto limit = [&](int k) { return lo + k < np ? P : P + len; };
 
-  uint32_t tmem = 0;
-  if (cnt > 0) {  // uniform over the CTA
-    if (warp == 9) {
-      ptx::tmem_alloc(ptx::smem_u32(tmem_holder), 512);
-      ptx::tmem_relinquish();
+  if (cnt == 0) {  // no keys: zeros, or an empty part
+    if (tid < nrow) {
+      const int tok = t_first + (row0 + tid) / G, h = g * G + (row0 + tid) % G;
+      if (parts.o) {
+        parts.lse[(int64_t)(parts.first + z) * parts.rows + (int64_t)tok * a.Hq + h] = -INFINITY;
+      } else {
+        E* dst = reinterpret_cast<E*>(a.out) + tok * a.o_ts + (int64_t)h * a.o_hs;
+#pragma unroll
+        for (int c = 0; c < D; c += 8)
+          *reinterpret_cast<uint4*>(dst + c) = make_uint4(0u, 0u, 0u, 0u);
+      }
     }
-    ptx::tc_fence_before();
-    __syncthreads();
-    ptx::tc_fence_after();
-    tmem = *tmem_holder;
+    return;
   }
 
+  if (warp == 9) {
+    ptx::tmem_alloc(ptx::smem_u32(tmem_holder), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+
   if (warp < 8) {
-    if (cnt > 0) ptx::reg_inc<TC_REG_SOFTMAX>();
+    ptx::reg_inc<TC_REG_SOFTMAX>();
     // ---------------------------------------------------------------- softmax
     const int t = warp >> 2;
     const int rr = row0 + tid;                  // tid < 256: both halves in order
@@ -220,7 +232,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
     float m = -INFINITY, l = 0.f;
     const bool half_on = t < halves;
     bool ok = true;
-    if (cnt > 0) {
+    {
       // this row of Q, K-major with the 128-byte swizzle
       uint8_t* qs = smem + t * L::TILE + (tid & 127) * 128;
       const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const E*>(a.q) +
@@ -238,7 +250,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
     const uint32_t ts = tmem + L::COL_S + t * 128 + lanes;
     const uint32_t tp = tmem + L::COL_P + t * L::STEP_P + lanes;
     const uint32_t to = tmem + L::COL_O + t * D + lanes;
-    if (half_on && cnt > 0) {
+    if (half_on) {
       constexpr float LOG2E = 1.4426950408889634f;
       const bool plain = a.cap == 0.f && a.slopes == nullptr && a.scale > 0.f;
       const float mul = plain ? a.scale * LOG2E : 1.f;
@@ -358,14 +370,9 @@ __global__ void __launch_bounds__(TC_NT, 1)
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
-        if (cnt > 0) {
-          ptx::tmem_ld_32x32b_x32(to + c, o);
-          ptx::tmem_ld_wait();
-          tc_regs(o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
-        }
+        ptx::tmem_ld_32x32b_x32(to + c, o);
+        ptx::tmem_ld_wait();
+        tc_regs(o);
         float* f = reinterpret_cast<float*>(o);
 #pragma unroll
         for (int e = 0; e < 32; ++e) f[e] = l == 0.f ? 0.f : f[e] * inv;
@@ -385,7 +392,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
         }
       }
     }
-  } else if (cnt > 0) {
+  } else {
     ptx::reg_dec<TC_REG_ISSUE>();
     if (warp == 8) {
     // -------------------------------------------------------------------- TMA
@@ -516,14 +523,12 @@ __global__ void __launch_bounds__(TC_NT, 1)
     }
     }
   }
-  if (cnt > 0) {
-    ptx::tc_fence_before();
-    __syncthreads();
-    if (tid == 0 && *abort_flag) record_device_error(DDQ_ERR_TIMEOUT);
-    if (warp == 9) {
-      ptx::tc_fence_after();
-      ptx::tmem_dealloc(tmem, 512);
-    }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) pg_error(a.c, DDQ_ERR_TIMEOUT);
+  if (warp == 9) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
   }
 }
 
