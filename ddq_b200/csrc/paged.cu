@@ -132,7 +132,7 @@ PgParts make_parts(void* ws, int64_t rows, int64_t D, int count) {
   float* o = static_cast<float*>(ws);
   return PgParts{o, o + (size_t)count * rows * D, rows, 0, count};
 }
-bool prefill_shape(int64_t T, int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
+bool attn_shape(int64_t T, int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
                    int64_t page_size, int64_t prefix_len) {
   return T > 0 && R > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && D > 0 && table_width > 0 &&
          page_size > 0 && prefix_len >= 0;
@@ -144,7 +144,7 @@ extern "C" size_t ddq_paged_prefill_attention_workspace_size(int64_t T, int64_t 
                                                              int64_t table_width,
                                                              int64_t page_size,
                                                              int64_t prefix_len) {
-  if (!prefill_shape(T, R, Hq, Hkv, D, table_width, page_size, prefix_len)) return 0;
+  if (!attn_shape(T, R, Hq, Hkv, D, table_width, page_size, prefix_len)) return 0;
   const int s = tc_splits(T, R, (int)Hq, (int)Hkv, prefix_len + table_width * page_size, true,
                           sm_count());
   return parts_bytes(T * Hq, D, s);
@@ -154,8 +154,9 @@ extern "C" size_t ddq_paged_decode_attention_workspace_size(int64_t B, int64_t H
                                                             int64_t D, int64_t table_width,
                                                             int64_t page_size,
                                                             int64_t prefix_len) {
-  (void)B, (void)Hq, (void)Hkv, (void)D, (void)table_width, (void)page_size, (void)prefix_len;
-  return 0;
+  if (!attn_shape(B, B, Hq, Hkv, D, table_width, page_size, prefix_len)) return 0;
+  return dc_plan(B, (int)Hq, (int)Hkv, (int)D, table_width * page_size, prefix_len, sm_count())
+      .bytes;
 }
 
 extern "C" int ddq_paged_prefill_attention(
@@ -209,11 +210,14 @@ extern "C" int ddq_paged_decode_attention(
                   block_table, table_stride, table_width, lens, scale, softcap, B, Hq, c.Hkv,
                   c.D);
   if (st) return st;
-  (void)workspace, (void)workspace_bytes;
+  const DcPlan plan = dc_plan(B, (int)Hq, c.Hkv, c.D, table_width << c.page_shift, prefix_len,
+                              sm_count());
+  if (!workspace || workspace_bytes < plan.bytes) return DDQ_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return DDQ_ERR_ALIGNMENT;
   if (!(c.err = device_error_word())) return DDQ_ERR_DEVICE;
   PgAttnArgs a{c, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
                block_table, table_stride, (int)table_width, lens, nullptr, nullptr, prefix_pages,
                (int)prefix_len, slopes, scale, softcap, (int)B, (int)B, (int)Hq};
-  return launch_paged_attention(a, cache->dtype == DDQ_DTYPE_BF16,
-                                reinterpret_cast<cudaStream_t>(stream));
+  return launch_paged_decode(a, cache->dtype == DDQ_DTYPE_BF16, workspace, plan,
+                             wait_timeout_ns(), reinterpret_cast<cudaStream_t>(stream));
 }

@@ -1,6 +1,14 @@
 // paged_tc.cu - paged attention of many query rows on the tcgen05 tensor cores:
 // the new tokens of ragged requests, and the rows of a decode batch over the
-// prefix that they share.  The mathematics is in paged_attn.cu.
+// prefix that they share.
+//
+// Row (t, h), key head g = h / (Hq / Hkv), at position p, attends the keys j of
+// its own request (and of the shared prefix, which comes first) with j < end:
+//   s_j = scale q . k_j          (capped: cap * tanh(s_j / cap))
+//   z_j = s_j - slope_h |p - j|
+//   o   = sum_j exp(z_j - m) v_j / sum_j exp(z_j - m),   m = max_j z_j
+// and o = 0 where there is no such key.  A prompt's row has
+// end = max(p + 1, prefix_len + min(bidir, len)), a decode row all keys.
 //
 // The G = Hq / Hkv query heads of a key/value head are packed with the tokens:
 // row rr of a request is token rr / G, head g G + rr % G, so that a tile of 256
@@ -530,6 +538,75 @@ __global__ void __launch_bounds__(TC_NT, 1)
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, 512);
   }
+}
+
+// Joins the parts of every row: o = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z -
+// max), in part order.  One warp per row.
+template <typename E, int D>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PgAttnArgs a, const PgParts p) {
+  using Ty = PgType<E>;
+  constexpr int DPL = D / 32;
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const int t = (int)(row / a.Hq), h = (int)(row % a.Hq);
+  if (a.cu && (t < a.cu[0] || t >= a.cu[a.R])) return;  // a padded row stays as it is
+  float mx = -INFINITY;
+  for (int z = lane; z < p.count; z += 32) mx = fmaxf(mx, p.lse[z * p.rows + row]);
+  mx = warp_max(mx);
+  float den = 0.f, o[DPL];
+#pragma unroll
+  for (int e = 0; e < DPL; ++e) o[e] = 0.f;
+  for (int z0 = 0; z0 < p.count; z0 += 32) {
+    const float ls = z0 + lane < p.count ? p.lse[(z0 + lane) * p.rows + row] : -INFINITY;
+    const float wl = ls == -INFINITY ? 0.f : exp2f(ls - mx);
+    for (int z = 0; z < min(32, p.count - z0); ++z) {
+      const float w = __shfl_sync(0xffffffffu, wl, z);
+      if (w == 0.f) continue;
+      const float* src = p.o + ((z0 + z) * p.rows + row) * D + lane * DPL;
+      float v[DPL];
+      if constexpr (DPL == 2)
+        *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+      else
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+      den += w;
+#pragma unroll
+      for (int e = 0; e < DPL; ++e) o[e] = fmaf(w, v[e], o[e]);
+    }
+  }
+  const float inv = den == 0.f ? 0.f : 1.f / den;  // NaN stays NaN
+  E* dst = reinterpret_cast<E*>(a.out) + t * a.o_ts + (int64_t)h * a.o_hs + lane * DPL;
+#pragma unroll
+  for (int e = 0; e < DPL; e += 2)
+    *reinterpret_cast<uint32_t*>(dst + e) = Ty::pack(o[e] * inv, o[e + 1] * inv);
+}
+
+int launch_paged_merge(const PgAttnArgs& a, bool bf16, const PgParts& parts, cudaStream_t s) {
+  const int64_t blocks = (parts.rows + 7) / 8;
+  if (blocks > 0x7fffffff) return DDQ_ERR_SHAPE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  cudaError_t e;
+  if (bf16)
+    e = a.c.D == 64 ? cudaLaunchKernelEx(&cfg, paged_merge_kernel<__nv_bfloat16, 64>, a, parts)
+                    : cudaLaunchKernelEx(&cfg, paged_merge_kernel<__nv_bfloat16, 128>, a, parts);
+  else
+    e = a.c.D == 64 ? cudaLaunchKernelEx(&cfg, paged_merge_kernel<__half, 64>, a, parts)
+                    : cudaLaunchKernelEx(&cfg, paged_merge_kernel<__half, 128>, a, parts);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return DDQ_ERR_LAUNCH;
+  }
+  return check_launch();
 }
 
 namespace {
