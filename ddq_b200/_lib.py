@@ -6,10 +6,11 @@ library is missing the first call raises; there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
-from .build import LIB_PATH
+from .build import LIB_PATH, TORCH_PATH
 
 _c_int64 = ctypes.c_int64
 _vp = ctypes.c_void_p
@@ -117,6 +118,34 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+_paged = None
+_PAGED_ENTRIES = ("ddq_plan_step", "ddq_paged_rope_kv",
+                  "ddq_paged_prefill_attention_workspace_size",
+                  "ddq_paged_decode_attention_workspace_size", "ddq_paged_prefill_attention",
+                  "ddq_paged_decode_attention", "ddq_status_string")
+
+
+def load_paged():
+    """The paged operators' CPython module, bound to the library's entries
+    (raises if either has not been built)."""
+    global _paged
+    if _paged is not None:
+        return _paged
+    lib = load()
+    with _lock:
+        if _paged is None:
+            if not os.path.exists(TORCH_PATH):
+                raise RuntimeError(
+                    f"ddq_b200: {TORCH_PATH} not found; build it with `python -m ddq_b200.build`")
+            import torch  # noqa: F401  (the libraries that the module links against)
+            spec = importlib.util.spec_from_file_location("_paged", TORCH_PATH)
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+            mod.bind(*(ctypes.cast(getattr(lib, name), _vp).value for name in _PAGED_ENTRIES))
+            _paged = mod
+    return _paged
 
 
 def status_string(status: int) -> str:

@@ -4,7 +4,8 @@ Every ``csrc/*.cu`` file is compiled for sm_100a only
 (``-gencode arch=compute_100a,code=sm_100a``) with relocatable device code
 (but for WHOLE_PROGRAM), in parallel, then device-linked into one shared library that exports the C ABI
 declared in ``include/ddq_b200.h``.  The library links the CUDA runtime
-statically and does not depend on torch.  Sources are rebuilt only when a
+statically and does not depend on torch; ``_paged.so`` beside it, host code on
+torch's headers, holds the tensor checks of the paged operators.  Sources are rebuilt only when a
 ``.cu``/``.cuh``/header file is newer than the library.
 
     python -m ddq_b200.build            # build if stale
@@ -27,6 +28,9 @@ INCLUDE = os.path.join(REPO_DIR, "include")
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libddq_b200.so")
+# the paged operators' checks and tensor handling as a CPython module on torch
+TORCH_SRC = os.path.join(CSRC, "torch_paged.cpp")
+TORCH_PATH = os.path.join(LIB_DIR, "_paged.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-rdc=true", "-Xcompiler", "-fPIC",
@@ -76,8 +80,38 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def build_torch(force: bool = False) -> str:
+    """The CPython module of the paged operators (host code only; it gets the
+    library's entry points at run time)."""
+    deps = [TORCH_SRC, os.path.abspath(__file__)] + glob.glob(os.path.join(INCLUDE, "*.h"))
+    if not force and os.path.exists(TORCH_PATH) and \
+            all(os.path.getmtime(TORCH_PATH) >= os.path.getmtime(p) for p in deps):
+        return TORCH_PATH
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    os.makedirs(LIB_DIR, exist_ok=True)
+    tmp = TORCH_PATH + ".tmp"
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-I", os.path.join(root, "include"),
+           "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I", sysconfig.get_paths()["include"], "-I", os.path.join(cuda, "include"), TORCH_SRC,
+           "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+           "-ltorch_python", "-o", tmp]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {TORCH_SRC}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_PATH)
+    return TORCH_PATH
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library if needed; return its path."""
+    """Compile the library (and the paged operators' module) if needed; return
+    the library's path."""
+    build_torch(force)
     if not force and not is_stale():
         return LIB_PATH
     os.makedirs(BUILD_DIR, exist_ok=True)
