@@ -94,6 +94,18 @@ __device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, uint64_t 
   return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, tmo, abort));
 }
 
+// One arrival for the warp, after all its lanes got here.
+__device__ __forceinline__ void tc_arrive(uint32_t bar, int lane) {
+  __syncwarp();
+  if (lane == 0) ptx::mbar_arrive(bar);
+}
+
+__device__ __forceinline__ float tc_max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 template <typename E, int D>
 __global__ void __launch_bounds__(TC_NT, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
@@ -125,11 +137,11 @@ __global__ void __launch_bounds__(TC_NT, 1)
       ptx::mbar_init(bar_full + 8 * s, 1);
       ptx::mbar_init(bar_empty + 8 * s, 1);
     }
-    ptx::mbar_init(bar_q, TC_ROWS);
+    ptx::mbar_init(bar_q, 8);  // warps
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(bar_s + 8 * t, 1);
-      ptx::mbar_init(bar_sfree + 8 * t, TC_HALF);
-      ptx::mbar_init(bar_p + 8 * t, TC_HALF);
+      ptx::mbar_init(bar_sfree + 8 * t, 4);
+      ptx::mbar_init(bar_p + 8 * t, 4);
       ptx::mbar_init(bar_pv + 8 * t, 1);
     }
     ptx::mbar_init(bar_drain, 1);
@@ -252,7 +264,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
       for (int c = 0; c < D / 8; ++c)
         *reinterpret_cast<uint4*>(qs + (c >> 3) * L::HB + (((c & 7) ^ (tid & 7)) << 4)) = v[c];
       ptx::fence_proxy_async_smem();
-      ptx::mbar_arrive(bar_q);
+      tc_arrive(bar_q, lane);
     }
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + L::COL_S + t * 128 + lanes;
@@ -281,7 +293,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
         for (int c = 0; c < 128; c += 32) tc_regs(u + c);
         if constexpr (SEP) {
           ptx::tc_fence_before();
-          ptx::mbar_arrive(bar_sfree + 8 * t);
+          tc_arrive(bar_sfree + 8 * t, lane);
         }
         float* s = reinterpret_cast<float*>(u);
         if (!plain) {  // to log2 units, capped and biased
@@ -311,12 +323,14 @@ __global__ void __launch_bounds__(TC_NT, 1)
         }
         float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
 #pragma unroll
-        for (int c = 4; c < 128; c += 4) {
-          x0 = fmaxf(x0, s[c]);
-          x1 = fmaxf(x1, s[c + 1]);
-          x2 = fmaxf(x2, s[c + 2]);
-          x3 = fmaxf(x3, s[c + 3]);
+        for (int c = 4; c < 124; c += 8) {
+          x0 = tc_max3(x0, s[c], s[c + 1]);
+          x1 = tc_max3(x1, s[c + 2], s[c + 3]);
+          x2 = tc_max3(x2, s[c + 4], s[c + 5]);
+          x3 = tc_max3(x3, s[c + 6], s[c + 7]);
         }
+        x0 = tc_max3(x0, s[124], s[125]);
+        x1 = tc_max3(x1, s[126], s[127]);
         const float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * mul;
         float alpha = 1.f;
         if (mx > m + TC_LAZY) {  // also the first keys of the row (m = -inf)
@@ -360,7 +374,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
         ptx::tmem_st_32x32b_x32(tp + 32, u + 32);
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
-        ptx::mbar_arrive(bar_p + 8 * t);
+        tc_arrive(bar_p + 8 * t, lane);
       }
       if (ok) ok = tc_wait(bar_pv + 8 * t, (uint32_t)(cnt - 1) & 1u, tmo, abort_flag);
       ptx::tc_fence_after();
@@ -447,80 +461,98 @@ __global__ void __launch_bounds__(TC_NT, 1)
     constexpr bool BF = sizeof(E) == 2 && !std::is_same<E, __half>::value;
     constexpr uint32_t id_qk = ptx::idesc_16_f32(TC_HALF, TC_KV, BF, false);
     constexpr uint32_t id_pv = ptx::idesc_16_f32(TC_HALF, D, BF, true);
+    // uniform copies: the loop below and every operand of its MMAs are the same
+    // for the warp, and the compiler can see it (an MMA whose descriptors come
+    // from vector registers took 130 cycles to issue)
+    const int cnt_u = __reduce_max_sync(0xffffffffu, cnt);
+    const int halves_u = __reduce_max_sync(0xffffffffu, halves);
+    const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
+    const uint32_t who = ptx::elect_one();
     const uint64_t dq = ptx::smem_desc_sw128(sbase);
     const uint64_t dk = ptx::smem_desc_sw128(sbase + L::OFF_RING);
     const uint64_t dv = ptx::smem_desc_sw128_mn(sbase + L::OFF_RING, L::HB);
     auto stage = [&](int k, int kv) { return (2 * k + kv) % L::ST; };
     auto wait_full = [&](int k, int kv) {
-      return tc_wait(bar_full + 8 * stage(k, kv),
-                            (uint32_t)((2 * k + kv) / L::ST) & 1u, tmo, abort_flag);
+      return tc_wait(bar_full + 8 * stage(k, kv), (uint32_t)((2 * k + kv) / L::ST) & 1u, tmo,
+                     abort_flag);
     };
     auto qk = [&](int k, int t) {
-      if (lane == 0) {
-        const uint64_t b0 = dk + (uint64_t)((stage(k, 0) * L::TILE) >> 4);
-        const uint64_t a0 = dq + (uint64_t)((t * L::TILE) >> 4);
+      const uint64_t b0 = dk + (uint64_t)((stage(k, 0) * L::TILE) >> 4);
+      const uint64_t a0 = dq + (uint64_t)((t * L::TILE) >> 4);
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) {
-          const uint64_t o = (uint64_t)(((e >> 2) * L::HB + (e & 3) * 32) >> 4);
-          ptx::mma_f16_ss(tmem + L::COL_S + t * 128, a0 + o, b0 + o, id_qk, e != 0 ? 1u : 0u);
-        }
-        ptx::mma_commit(bar_s + 8 * t);
-        if (t == halves - 1) ptx::mma_commit(bar_empty + 8 * stage(k, 0));
+      for (int e = 0; e < D / 16; ++e) {
+        const uint64_t o = (uint64_t)(((e >> 2) * L::HB + (e & 3) * 32) >> 4);
+        ptx::mma_f16_ss_if(who, tm + L::COL_S + t * 128, a0 + o, b0 + o, id_qk,
+                           e != 0 ? 1u : 0u);
       }
-      __syncwarp();
+      ptx::mma_commit_if(who, bar_s + 8 * t);
+      if (t == halves_u - 1) ptx::mma_commit_if(who, bar_empty + 8 * stage(k, 0));
     };
     auto pv = [&](int k, int t) {
-      if (lane == 0) {
-        const uint64_t b0 = dv + (uint64_t)((stage(k, 1) * L::TILE) >> 4);
-        const uint32_t p0 = tmem + L::COL_P + t * L::STEP_P;
+      const uint64_t b0 = dv + (uint64_t)((stage(k, 1) * L::TILE) >> 4);
+      const uint32_t p0 = tm + L::COL_P + t * L::STEP_P;
 #pragma unroll
-        for (int e = 0; e < TC_KV / 16; ++e)
-          ptx::mma_f16_ts(tmem + L::COL_O + t * D, p0 + e * 8, b0 + (uint64_t)((e * 2048) >> 4),
-                          id_pv, (k | e) != 0 ? 1u : 0u);
-        ptx::mma_commit(bar_pv + 8 * t);
-        if (t == halves - 1) ptx::mma_commit(bar_empty + 8 * stage(k, 1));
-      }
+      for (int e = 0; e < TC_KV / 16; ++e)
+        ptx::mma_f16_ts_if(who, tm + L::COL_O + t * D, p0 + e * 8,
+                           b0 + (uint64_t)((e * 2048) >> 4), id_pv, (k | e) != 0 ? 1u : 0u);
+      ptx::mma_commit_if(who, bar_pv + 8 * t);
+      if (t == halves_u - 1) ptx::mma_commit_if(who, bar_empty + 8 * stage(k, 1));
+    };
+    // V's rows behind the last key may hold anything (or were not loaded): their
+    // weights are zero, and 0 x NaN is NaN
+    auto clear_tail = [&](int k) {
+      const int have = limit(k) - key0(k);
+      if (have >= TC_KV) return;
+      uint8_t* vs = smem + L::OFF_RING + stage(k, 1) * L::TILE;
+      for (int x = have * 8 + lane; x < TC_KV * 8; x += 32)
+#pragma unroll
+        for (int hb = 0; hb < D / 64; ++hb)
+          *reinterpret_cast<uint4*>(vs + hb * L::HB + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+      ptx::fence_proxy_async_smem();
       __syncwarp();
     };
+    const bool two = halves_u == 2;
     bool ok = tc_wait(bar_q, 0, tmo, abort_flag) && wait_full(0, 0);
     ptx::tc_fence_after();
-    if (ok)
-      for (int t = 0; t < halves; ++t) qk(0, t);
-    for (int k = 0; k < cnt && ok; ++k) {
-      for (int t = 0; t < halves && ok; ++t) {
-        if (SEP && k + 1 < cnt) {
-          if (t == 0) ok = wait_full(k + 1, 0);
-          ok = ok && tc_wait(bar_sfree + 8 * t, (uint32_t)k & 1u, tmo, abort_flag);
-          if (!ok) break;
-          ptx::tc_fence_after();
-          qk(k + 1, t);
-        }
-        if (t == 0) {
-          ok = wait_full(k, 1);
-          if (!ok) break;
-          const int have = limit(k) - key0(k);
-          if (have < TC_KV) {
-            // the rows behind the last key may hold anything (or were not
-            // loaded): their weights are zero, and 0 x NaN is NaN
-            uint8_t* vs = smem + L::OFF_RING + stage(k, 1) * L::TILE;
-            for (int x = have * 8 + lane; x < TC_KV * 8; x += 32)
-#pragma unroll
-              for (int hb = 0; hb < D / 64; ++hb)
-                *reinterpret_cast<uint4*>(vs + hb * L::HB + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-          }
-        }
-        ok = tc_wait(bar_p + 8 * t, (uint32_t)k & 1u, tmo, abort_flag);
+    if (ok) {
+      qk(0, 0);
+      if (two) qk(0, 1);
+    }
+    for (int k = 0; k < cnt_u; ++k) {
+      if (!ok) break;
+      const bool more = k + 1 < cnt_u;
+      const uint32_t par = (uint32_t)k & 1u;
+      if (SEP && more) {
+        ok = wait_full(k + 1, 0) && tc_wait(bar_sfree, par, tmo, abort_flag);
         if (!ok) break;
         ptx::tc_fence_after();
-        pv(k, t);
-        if (!SEP && k + 1 < cnt) {
-          if (t == 0) ok = wait_full(k + 1, 0);
+        qk(k + 1, 0);
+      }
+      ok = wait_full(k, 1);
+      if (!ok) break;
+      clear_tail(k);
+      ok = tc_wait(bar_p, par, tmo, abort_flag);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      pv(k, 0);
+      if (!SEP && more) {
+        ok = wait_full(k + 1, 0);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        qk(k + 1, 0);
+      }
+      if (two) {
+        if (SEP && more) {
+          ok = tc_wait(bar_sfree + 8, par, tmo, abort_flag);
           if (!ok) break;
           ptx::tc_fence_after();
-          qk(k + 1, t);
+          qk(k + 1, 1);
         }
+        ok = tc_wait(bar_p + 8, par, tmo, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        pv(k, 1);
+        if (!SEP && more) qk(k + 1, 1);
       }
     }
     if (!ok) {
