@@ -81,12 +81,15 @@ struct PgType<__nv_bfloat16> {
 
 // Keys of request r in its own pages: the length, never more than its table
 // row holds (a longer one is an error of the caller's, recorded).
-__device__ __forceinline__ int pg_len(const PgAttnArgs& a, int r) {
-  const int n = a.lens[r] < 0 ? 0 : a.lens[r];
+__device__ __forceinline__ int pg_clamp_len(const PgAttnArgs& a, int n) {
   const int64_t hold = (int64_t)a.width << a.c.page_shift;
-  if (n <= hold) return n;
+  if (n <= hold) return n < 0 ? 0 : n;
   pg_error(a.c, DDQ_ERR_PAGE);
   return (int)hold;
+}
+
+__device__ __forceinline__ int pg_len(const PgAttnArgs& a, int r) {
+  return pg_clamp_len(a, a.lens[r]);
 }
 
 // A page number as the tables hold it, -1 (recorded) for one outside the pool.

@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   const uint32_t sbase = ptx::smem_u32(smem);
-  __shared__ int found[2], wsum[TC_NT / 32];
+  __shared__ int found[6], wsum[TC_NT / 32];  // request, tile, first row, rows, keys, bidir
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.Hq / a.c.Hkv, g = blockIdx.y, z = blockIdx.z;
 
@@ -128,9 +128,10 @@ __global__ void __launch_bounds__(TC_NT, 1)
   const uint32_t bar_s = bar_q + 8;         // [2] scores ready
   const uint32_t bar_sfree = bar_s + 16;    // [2] scores read (SEP)
   const uint32_t bar_p = bar_sfree + 16;    // [2] weights ready
-  const uint32_t bar_pv = bar_p + 16;       // [2] PV done
+  const uint32_t bar_p2 = bar_p + 16;       // [2] ... of the tile's second 64 keys
+  const uint32_t bar_pv = bar_p2 + 16;      // [2] PV done
   const uint32_t bar_drain = bar_pv + 16;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_BAR + 8 * (2 * L::ST + 10));
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_BAR + 8 * (2 * L::ST + 12));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   if (tid == 0) {
     for (int s = 0; s < L::ST; ++s) {
@@ -142,6 +143,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
       ptx::mbar_init(bar_s + 8 * t, 1);
       ptx::mbar_init(bar_sfree + 8 * t, 4);
       ptx::mbar_init(bar_p + 8 * t, 4);
+      ptx::mbar_init(bar_p2 + 8 * t, 4);
       ptx::mbar_init(bar_pv + 8 * t, 1);
     }
     ptx::mbar_init(bar_drain, 1);
@@ -155,16 +157,19 @@ __global__ void __launch_bounds__(TC_NT, 1)
   ptx::pdl_launch_dependents();
   __syncthreads();
 
-  // ---- the request and the tile of this CTA
+  // ---- the request and the tile of this CTA: requests and their tiles from the
+  // last to the first, so that the CTAs that start last have the fewest keys
   int r = 0, tile = blockIdx.x, t_first = 0, n = a.T;
   if (a.cu) {
     int run = 0;
     for (int base = 0; base < a.R; base += TC_NT) {
-      const int rr = base + tid;
-      int c0 = 0, cn = 0;
-      if (rr < a.R) {
+      const int rr = a.R - 1 - (base + tid);
+      int c0 = 0, cn = 0, ln = 0, bd = 0;
+      if (rr >= 0) {  // one round of loads; the CTA's request is among them
         c0 = a.cu[rr];
         cn = a.cu[rr + 1] - c0;
+        ln = a.lens[rr];
+        if (a.bidir) bd = a.bidir[rr];
         if (c0 < 0 || c0 >= a.T || cn < 0) cn = 0;
         cn = min(cn, a.T - c0);
       }
@@ -186,7 +191,11 @@ __global__ void __launch_bounds__(TC_NT, 1)
       s += before;
       if (tile < s && tile >= s - tiles) {
         found[0] = rr;
-        found[1] = tile - (s - tiles);
+        found[1] = s - 1 - tile;
+        found[2] = c0;
+        found[3] = cn;
+        found[4] = pg_clamp_len(a, ln);
+        found[5] = bd;
       }
       __syncthreads();
       if (found[0] >= 0) break;
@@ -194,12 +203,12 @@ __global__ void __launch_bounds__(TC_NT, 1)
     r = found[0];
     if (r < 0) return;  // the grid covers the most tiles that T rows can make
     tile = found[1];
-    t_first = a.cu[r];
-    n = min(a.cu[r + 1] - t_first, a.T - t_first);
+    t_first = found[2];
+    n = found[3];
   }
   const int P = a.prefix_len;
-  const int len = a.cu ? pg_len(a, r) : 0;
-  const int least = a.cu ? (a.bidir ? P + min(a.bidir[r], len) : 0) : P;
+  const int len = a.cu ? found[4] : 0;
+  const int least = a.cu ? (a.bidir ? P + min(found[5], len) : 0) : P;
   const int row0 = tile * TC_ROWS, nrow = min(TC_ROWS, n * G - row0);
   const int halves = nrow > TC_HALF ? 2 : 1;
   // keys of the row of token i: those below end(i); the last row has the most
@@ -252,17 +261,32 @@ __global__ void __launch_bounds__(TC_NT, 1)
     float m = -INFINITY, l = 0.f;
     const bool half_on = t < halves;
     bool ok = true;
+    // This warp's 32 rows of Q, K-major with the 128-byte swizzle, and later its
+    // rows of the output, through the same shared memory (Q is done with when the
+    // last scores are there): D / 8 lanes read or write a row together.  (One
+    // thread per row touched 32 lines an access: 13 of 82 thousand cycles of a
+    // CTA of 16 tiles.)
+    uint8_t* const rows = smem + t * L::TILE + (warp & 3) * 32 * 128;
+    auto piece = [&](int row, int c) {  // 16-byte piece c of 64-element block 0
+      return row * 128 + ((c ^ (row & 7)) << 4);
+    };
     {
-      // this row of Q, K-major with the 128-byte swizzle
-      uint8_t* qs = smem + t * L::TILE + (tid & 127) * 128;
-      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const E*>(a.q) +
-                                                        tok * a.q_ts + (int64_t)h * a.q_hs);
-      uint4 v[D / 8];
+      const int64_t q_off = real ? tok * a.q_ts + (int64_t)h * a.q_hs : -1;
+      constexpr int LPR = D / 8;  // lanes per row
+      uint4 v[LPR];
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) v[c] = real ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+      for (int e = 0; e < LPR; ++e) {
+        const int64_t off = __shfl_sync(0xffffffffu, q_off, e * (32 / LPR) + lane / LPR);
+        v[e] = make_uint4(0u, 0u, 0u, 0u);
+        if (off >= 0)
+          v[e] = *reinterpret_cast<const uint4*>(reinterpret_cast<const E*>(a.q) + off +
+                                                 8 * (lane % LPR));
+      }
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c)
-        *reinterpret_cast<uint4*>(qs + (c >> 3) * L::HB + (((c & 7) ^ (tid & 7)) << 4)) = v[c];
+      for (int e = 0; e < LPR; ++e) {
+        const int row = e * (32 / LPR) + lane / LPR, c = lane % LPR;
+        *reinterpret_cast<uint4*>(rows + (c >> 3) * L::HB + piece(row, c & 7)) = v[e];
+      }
       ptx::fence_proxy_async_smem();
       tc_arrive(bar_q, lane);
     }
@@ -356,25 +380,29 @@ __global__ void __launch_bounds__(TC_NT, 1)
           }
         }
         const float mu = m == -INFINITY ? 0.f : m;
-        float l0 = 0.f, l1 = 0.f;
+        // P of 64 keys at a time, so that PV starts while the rest is made
 #pragma unroll
-        for (int c = 0; c < 128; c += 2) {
-          const float p0 = tc_exp2(fmaf(s[c], mul, -mu)), p1 = tc_exp2(fmaf(s[c + 1], mul, -mu));
-          l0 += p0;
-          l1 += p1;
-          u[c >> 1] = Ty::pack(p0, p1);
+        for (int hf = 0; hf < 2; ++hf) {
+          float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+          for (int c = 64 * hf; c < 64 * hf + 64; c += 2) {
+            const float p0 = tc_exp2(fmaf(s[c], mul, -mu)), p1 = tc_exp2(fmaf(s[c + 1], mul, -mu));
+            l0 += p0;
+            l1 += p1;
+            u[c >> 1] = Ty::pack(p0, p1);
+          }
+          l += l0 + l1;
+          if (SEP && hf == 0 && k > 0) {  // P of the tile before has been read
+            ok = tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
+            if (!ok) break;
+            ptx::tc_fence_after();
+          }
+          ptx::tmem_st_32x32b_x32(tp + 32 * hf, u + 32 * hf);
+          ptx::tmem_st_wait();
+          ptx::tc_fence_before();
+          tc_arrive((hf ? bar_p2 : bar_p) + 8 * t, lane);
         }
-        l += l0 + l1;
-        if (SEP && k > 0) {  // P of the tile before has been read
-          ok = tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
-          if (!ok) break;
-          ptx::tc_fence_after();
-        }
-        ptx::tmem_st_32x32b_x32(tp, u);
-        ptx::tmem_st_32x32b_x32(tp + 32, u + 32);
-        ptx::tmem_st_wait();
-        ptx::tc_fence_before();
-        tc_arrive(bar_p + 8 * t, lane);
+        if (!ok) break;
       }
       if (ok) ok = tc_wait(bar_pv + 8 * t, (uint32_t)(cnt - 1) & 1u, tmo, abort_flag);
       ptx::tc_fence_after();
@@ -383,12 +411,12 @@ __global__ void __launch_bounds__(TC_NT, 1)
     // loads; a half without rows, and a row behind the last, stores nothing.
     if (half_on && ok) {
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: 0; NaN stays
-      E* dst = reinterpret_cast<E*>(a.out) + tok * a.o_ts + (int64_t)h * a.o_hs;
-      const int64_t prow = (int64_t)tok * a.Hq + h;
-      float* po = parts.o ? parts.o + ((int64_t)(parts.first + z) * parts.rows + prow) * D : nullptr;
-      if (parts.o && real)
-        parts.lse[(int64_t)(parts.first + z) * parts.rows + prow] =
-            l == 0.f ? -INFINITY : m + log2f(l);
+      const int64_t prow = (int64_t)(parts.first + z) * parts.rows + (int64_t)tok * a.Hq + h;
+      const bool part = parts.o != nullptr;
+      if (part && real) parts.lse[prow] = l == 0.f ? -INFINITY : m + log2f(l);
+      // offset of this thread's row; -1: nothing to store
+      const int64_t off = !real ? -1 : part ? (l == 0.f ? -1 : prow * D)
+                                            : tok * a.o_ts + (int64_t)h * a.o_hs;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -398,20 +426,33 @@ __global__ void __launch_bounds__(TC_NT, 1)
         float* f = reinterpret_cast<float*>(o);
 #pragma unroll
         for (int e = 0; e < 32; ++e) f[e] = l == 0.f ? 0.f : f[e] * inv;
-        if (real && po) {
-          if (l != 0.f) {
+        if (part) {  // 32 columns of fp32: 128 bytes a row
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(po + c + e) =
-                  make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-          }
-        } else if (real) {
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(rows + piece(lane, e)) =
+                make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+        } else {     // 64 columns
 #pragma unroll
-          for (int e = 0; e < 32; e += 8)
-            *reinterpret_cast<uint4*>(dst + c + e) =
-                make_uint4(Ty::pack(f[e], f[e + 1]), Ty::pack(f[e + 2], f[e + 3]),
-                           Ty::pack(f[e + 4], f[e + 5]), Ty::pack(f[e + 6], f[e + 7]));
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(rows + piece(lane, (c & 32) / 8 + e)) = make_uint4(
+                Ty::pack(f[8 * e], f[8 * e + 1]), Ty::pack(f[8 * e + 2], f[8 * e + 3]),
+                Ty::pack(f[8 * e + 4], f[8 * e + 5]), Ty::pack(f[8 * e + 6], f[8 * e + 7]));
+          if ((c & 32) == 0) continue;
         }
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {  // 8 lanes a row
+          const int row = 4 * e + (lane >> 3);
+          const int64_t ro = __shfl_sync(0xffffffffu, off, row);
+          const uint4 v = *reinterpret_cast<const uint4*>(rows + piece(row, lane & 7));
+          if (ro < 0) continue;
+          if (part)
+            *reinterpret_cast<uint4*>(parts.o + ro + c + 4 * (lane & 7)) = v;
+          else
+            *reinterpret_cast<uint4*>(reinterpret_cast<E*>(a.out) + ro + (c & ~63) +
+                                      8 * (lane & 7)) = v;
+        }
+        __syncwarp();
       }
     }
   } else {
@@ -424,23 +465,28 @@ __global__ void __launch_bounds__(TC_NT, 1)
     const int* own = a.table + (int64_t)r * a.table_stride;
     int g_ring = 0;
     bool ok = true;
-    for (int k = 0; k < cnt && ok; ++k) {
+    // page number and row of this lane's box of tile k (looked up a tile ahead:
+    // the table read takes as long as a tile's softmax)
+    auto look = [&](int k, int& page, int& prow) {
       const bool shared = lo + k < np;
       const int off = (shared ? (lo + k) : (lo + k - np)) * TC_KV + box * br;  // in its list
-      const int have = limit(k) - key0(k);
-      bool mine = dh < D / 64 && box * br < have;
-      int page = 0;
-      if (mine) {
-        page = pg_check(a.c, (shared ? a.prefix_pages : own)[off >> a.c.page_shift]);
-        mine = page >= 0;
-      }
-      const int prow = off & ((1 << a.c.page_shift) - 1);
+      prow = off & ((1 << a.c.page_shift) - 1);
+      page = -1;
+      if (k >= cnt || dh >= D / 64 || box * br >= limit(k) - key0(k)) return false;
+      page = (shared ? a.prefix_pages : own)[off >> a.c.page_shift];
+      return true;
+    };
+    int page, prow;
+    bool mine = look(0, page, prow);
+    for (int k = 0; k < cnt && ok; ++k) {
+      int page1, prow1;
+      const bool mine1 = look(k + 1, page1, prow1);
+      if (mine) mine = pg_check(a.c, page) >= 0;
       const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, mine)) * br * 128u;
 #pragma unroll
       for (int kv = 0; kv < 2 && ok; ++kv, ++g_ring) {
         const int s = g_ring % L::ST;
-        ok = tc_wait(bar_empty + 8 * s, ((uint32_t)(g_ring / L::ST) & 1u) ^ 1u, tmo,
-                            abort_flag);
+        ok = tc_wait(bar_empty + 8 * s, ((uint32_t)(g_ring / L::ST) & 1u) ^ 1u, tmo, abort_flag);
         if (!ok) break;
         if (lane == 0) ptx::mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
         __syncwarp();
@@ -448,6 +494,9 @@ __global__ void __launch_bounds__(TC_NT, 1)
           ptx::tma_load_4d(sbase + L::OFF_RING + s * L::TILE + dh * L::HB + box * br * 128,
                            kv ? &tm_v : &tm_k, dh * 64, prow, g, page, bar_full + 8 * s);
       }
+      mine = mine1;
+      page = page1;
+      prow = prow1;
     }
     if (!ok) {  // copies in flight land before the shared memory goes
       for (int q = g_ring > L::ST ? g_ring - L::ST : 0; q < g_ring; ++q) {
@@ -488,13 +537,14 @@ __global__ void __launch_bounds__(TC_NT, 1)
       ptx::mma_commit_if(who, bar_s + 8 * t);
       if (t == halves_u - 1) ptx::mma_commit_if(who, bar_empty + 8 * stage(k, 0));
     };
-    auto pv = [&](int k, int t) {
+    auto pv = [&](int k, int t, int hf) {  // 64 keys
       const uint64_t b0 = dv + (uint64_t)((stage(k, 1) * L::TILE) >> 4);
       const uint32_t p0 = tm + L::COL_P + t * L::STEP_P;
 #pragma unroll
-      for (int e = 0; e < TC_KV / 16; ++e)
+      for (int e = 4 * hf; e < 4 * hf + 4; ++e)
         ptx::mma_f16_ts_if(who, tm + L::COL_O + t * D, p0 + e * 8,
                            b0 + (uint64_t)((e * 2048) >> 4), id_pv, (k | e) != 0 ? 1u : 0u);
+      if (hf == 0) return;
       ptx::mma_commit_if(who, bar_pv + 8 * t);
       if (t == halves_u - 1) ptx::mma_commit_if(who, bar_empty + 8 * stage(k, 1));
     };
@@ -534,7 +584,11 @@ __global__ void __launch_bounds__(TC_NT, 1)
       ok = tc_wait(bar_p, par, tmo, abort_flag);
       if (!ok) break;
       ptx::tc_fence_after();
-      pv(k, 0);
+      pv(k, 0, 0);
+      ok = tc_wait(bar_p2, par, tmo, abort_flag);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      pv(k, 0, 1);
       if (!SEP && more) {
         ok = wait_full(k + 1, 0);
         if (!ok) break;
@@ -551,7 +605,11 @@ __global__ void __launch_bounds__(TC_NT, 1)
         ok = tc_wait(bar_p + 8, par, tmo, abort_flag);
         if (!ok) break;
         ptx::tc_fence_after();
-        pv(k, 1);
+        pv(k, 1, 0);
+        ok = tc_wait(bar_p2 + 8, par, tmo, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        pv(k, 1, 1);
         if (!SEP && more) qk(k + 1, 1);
       }
     }
