@@ -87,11 +87,74 @@ __device__ __forceinline__ void tc_regs(uint32_t* r) {  // the loads above are c
                    "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
-// mbar_wait with one answer for the warp: the TMEM loads and stores after it
-// need all lanes, also when a wait gives up.
-__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, uint64_t tmo,
+// Two fp32 values in a register pair and the packed operations on them (half the
+// issue slots).
+struct TcF2 {
+  uint64_t v;
+};
+__device__ __forceinline__ TcF2 tc_pk(float a, float b) {
+  TcF2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void tc_un(TcF2 x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+}
+__device__ __forceinline__ TcF2 tc_fma2(TcF2 a, TcF2 b, TcF2 c) {
+  TcF2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ TcF2 tc_mul2(TcF2 a, TcF2 b) {
+  TcF2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ TcF2 tc_add2(TcF2 a, TcF2 b) {
+  TcF2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
+// 2^x for x <= 8 on the FMA pipe: x = n + f with n the nearest integer (adding
+// 1.5 2^23 leaves it in the low bits), 2^f by the minimax polynomial of degree 4
+// on [-1/2, 1/2] (Remez, relative error 2^-18.5: 2^-7 of the rounding of a
+// weight to 11 bits), n added to the exponent field.  Below 2^-126: 2^-126.
+__device__ __forceinline__ TcF2 tc_poly_exp2(float x0, float x1) {
+  constexpr float M = 12582912.f;
+  const TcF2 x = tc_pk(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const TcF2 t = tc_add2(x, tc_pk(M, M));
+  const TcF2 f = tc_add2(x, tc_mul2(tc_add2(t, tc_pk(-M, -M)), tc_pk(-1.f, -1.f)));
+  TcF2 p = tc_fma2(f, tc_pk(0x1.3997d6p-7f, 0x1.3997d6p-7f), tc_pk(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+  p = tc_fma2(p, f, tc_pk(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  p = tc_fma2(p, f, tc_pk(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  p = tc_fma2(p, f, tc_pk(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  float p0, p1, t0, t1;
+  tc_un(p, p0, p1);
+  tc_un(t, t0, t1);
+  return tc_pk(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23)),
+               __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
+}
+
+// Wait for a phase of a barrier, bounded like ptx::mbar_wait, but the caller goes
+// on in either case: after a wait that gave up (abort set, DDQ_ERR_TIMEOUT at the
+// end) every later one returns at once, the loops run out on whatever the
+// buffers hold, and no lane leaves its warp in between.  A wait on a phase that
+// is complete costs 55 cycles this way; with an answer for the warp to branch on
+// it cost 106, six times per pair of tiles on the path from P to the next S.
+__device__ __forceinline__ void tc_wait_slow(uint32_t bar, uint32_t parity, uint64_t tmo,
+                                          volatile int* abort) {
+  const long long t0 = clock64();
+  while (!*abort) {
+    for (int n = 0; n < 64; ++n)
+      if (ptx::mbar_try_wait_now(bar, parity)) return;
+    if (clock64() - t0 > (long long)(tmo * 2ull)) *abort = 1;
+  }
+}
+__device__ __forceinline__ void tc_wait(uint32_t bar, uint32_t parity, uint64_t tmo,
                                         volatile int* abort) {
-  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, tmo, abort));
+  if (!ptx::mbar_try_wait_now(bar, parity)) tc_wait_slow(bar, parity, tmo, abort);
+  __syncwarp();
 }
 
 // One arrival for the warp, after all its lanes got here.
@@ -256,11 +319,12 @@ __global__ void __launch_bounds__(TC_NT, 1)
     const bool real = tid < nrow;
     const int i = real ? rr / G : 0, h = g * G + (real ? rr % G : 0);
     const int tok = t_first + i;
-    const int end = real ? end_of(i) : 0;
+    // a row behind the last takes part unmasked (its Q is zero, its result is not
+    // stored): a warp of such rows has no slower tiles than the others
+    const int end = real ? end_of(i) : 0x7fffffff;
     const int pos = a.cu ? P + len - n + i : P + pg_len(a, real ? tok : 0) - 1;
     float m = -INFINITY, l = 0.f;
     const bool half_on = t < halves;
-    bool ok = true;
     // This warp's 32 rows of Q, K-major with the 128-byte swizzle, and later its
     // rows of the output, through the same shared memory (Q is done with when the
     // last scores are there): D / 8 lanes read or write a row together.  (One
@@ -301,115 +365,155 @@ __global__ void __launch_bounds__(TC_NT, 1)
       const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.f;
       for (int k = 0; k < cnt; ++k) {
         const int j0 = key0(k);
-        ok = tc_wait(bar_s + 8 * t, (uint32_t)k & 1u, tmo, abort_flag);
+        const int lim = min(end, limit(k)) - j0;  // keys of this tile that the row attends
+        const bool full = __all_sync(0xffffffffu, lim >= TC_KV);
+        tc_wait(bar_s + 8 * t, (uint32_t)k & 1u, tmo, abort_flag);
         // (P in S's place: the PV of the tile before is done too, as its MMAs
         // were issued before those of S; its barrier is waited for here so that
         // no phase of it is skipped)
-        if (!SEP && ok && k > 0)
-          ok = tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
-        if (!ok) break;
+        if (!SEP && k > 0) tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
         ptx::tc_fence_after();
-        uint32_t u[128];
+        // The row passes through registers 64 scores at a time, twice (a TMEM load
+        // of 64 columns takes 25 cycles): once for the maximum, once for the
+        // weights.  Loops, not 128 scores unrolled: the code of a tile in
+        // straight lines (16 KB a variant) kept the instruction caches busy, and
+        // the MMA warp waited hundreds of cycles for its next instruction.
+        const bool back = !plain || !full;  // scores changed on the way: put back
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t u[64];
+          float* s = reinterpret_cast<float*>(u);
+          ptx::tmem_ld_32x32b_x32(ts + 64 * hf, u);
+          ptx::tmem_ld_32x32b_x32(ts + 64 * hf + 32, u + 32);
+          ptx::tmem_ld_wait();
+          tc_regs(u);
+          tc_regs(u + 32);
+          if (back) {
+            if (!plain) {  // to log2 units, capped and biased
+              if (a.cap > 0.f) {
+                // cap tanh(y / cap) = cap - 2 cap / (exp(2 y / cap) + 1): an absolute
+                // error of a few 2^-23 cap, also where the exponential overflows
+                const float kk = 2.f * LOG2E * a.scale / a.cap, A = a.cap * LOG2E;
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) ptx::tmem_ld_32x32b_x32(ts + c, u + c);
-        ptx::tmem_ld_wait();
+                for (int c = 0; c < 64; ++c)
+                  s[c] = fmaf(-2.f * A, tc_rcp(tc_exp2(s[c] * kk) + 1.f), A);
+              } else {
+                const float kk = a.scale * LOG2E;
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) tc_regs(u + c);
-        if constexpr (SEP) {
-          ptx::tc_fence_before();
-          tc_arrive(bar_sfree + 8 * t, lane);
-        }
-        float* s = reinterpret_cast<float*>(u);
-        if (!plain) {  // to log2 units, capped and biased
-          if (a.cap > 0.f) {
-            // cap tanh(y / cap) = cap - 2 cap / (exp(2 y / cap) + 1): an absolute
-            // error of a few 2^-23 cap, also where the exponential overflows
-            const float kk = 2.f * LOG2E * a.scale / a.cap, A = a.cap * LOG2E;
+                for (int c = 0; c < 64; ++c) s[c] *= kk;
+              }
+              if (a.slopes) {
+                const float d0 = (float)(pos - j0 - 64 * hf);
 #pragma unroll
-            for (int c = 0; c < 128; ++c)
-              s[c] = fmaf(-2.f * A, tc_rcp(tc_exp2(s[c] * kk) + 1.f), A);
-          } else {
-            const float kk = a.scale * LOG2E;
+                for (int c = 0; c < 64; ++c) s[c] = fmaf(-slope, fabsf(d0 - (float)c), s[c]);
+              }
+            }
+            if (!full) {
+              const int lh = lim - 64 * hf;
 #pragma unroll
-            for (int c = 0; c < 128; ++c) s[c] *= kk;
+              for (int c = 0; c < 64; ++c)
+                if (c >= lh) s[c] = -INFINITY;
+            }
+            ptx::tmem_st_32x32b_x32(ts + 64 * hf, u);
+            ptx::tmem_st_32x32b_x32(ts + 64 * hf + 32, u + 32);
           }
-          if (a.slopes) {
-            const float d0 = (float)(pos - j0);
+          float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
 #pragma unroll
-            for (int c = 0; c < 128; ++c) s[c] = fmaf(-slope, fabsf(d0 - (float)c), s[c]);
+          for (int c = 4; c < 60; c += 8) {
+            x0 = tc_max3(x0, s[c], s[c + 1]);
+            x1 = tc_max3(x1, s[c + 2], s[c + 3]);
+            x2 = tc_max3(x2, s[c + 4], s[c + 5]);
+            x3 = tc_max3(x3, s[c + 6], s[c + 7]);
           }
+          x0 = tc_max3(x0, s[60], s[61]);
+          x1 = tc_max3(x1, s[62], s[63]);
+          mx = tc_max3(mx, fmaxf(x0, x1), fmaxf(x2, x3));
         }
-        const int lim = min(end, limit(k)) - j0;  // keys of this tile that the row attends
-        if (!__all_sync(0xffffffffu, lim >= TC_KV)) {
-#pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c >= lim) s[c] = -INFINITY;
-        }
-        float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
-#pragma unroll
-        for (int c = 4; c < 124; c += 8) {
-          x0 = tc_max3(x0, s[c], s[c + 1]);
-          x1 = tc_max3(x1, s[c + 2], s[c + 3]);
-          x2 = tc_max3(x2, s[c + 4], s[c + 5]);
-          x3 = tc_max3(x3, s[c + 6], s[c + 7]);
-        }
-        x0 = tc_max3(x0, s[124], s[125]);
-        x1 = tc_max3(x1, s[126], s[127]);
-        const float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * mul;
-        float alpha = 1.f;
-        if (mx > m + TC_LAZY) {  // also the first keys of the row (m = -inf)
-          if (m != -INFINITY) alpha = tc_exp2(m - mx);
-          m = mx;
-          l *= alpha;
-        }
-        if (k > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-          if constexpr (SEP) {
-            ok = tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
-            if (!ok) break;
-            ptx::tc_fence_after();
+        if (back) ptx::tmem_st_wait();
+        mx *= mul;
+        if (__any_sync(0xffffffffu, mx > m + TC_LAZY)) {
+          float alpha = 1.f;
+          if (mx > m + TC_LAZY) {  // also the first keys of the row (m = -inf)
+            if (m != -INFINITY) alpha = tc_exp2(m - mx);
+            m = mx;
+            l *= alpha;
           }
+          if (k > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+            if constexpr (SEP) {
+              tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
+              ptx::tc_fence_after();
+            }
 #pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            ptx::tmem_ld_32x32b_x32(to + c, o);
-            ptx::tmem_ld_wait();
-            tc_regs(o);
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              ptx::tmem_ld_32x32b_x32(to + c, o);
+              ptx::tmem_ld_wait();
+              tc_regs(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            ptx::tmem_st_32x32b_x32(to + c, o);
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              ptx::tmem_st_32x32b_x32(to + c, o);
+            }
           }
         }
         const float mu = m == -INFINITY ? 0.f : m;
-        // P of 64 keys at a time, so that PV starts while the rest is made
+        const TcF2 mul2 = tc_pk(mul, mul), mu2 = tc_pk(-mu, -mu);
+        TcF2 la = tc_pk(0.f, 0.f), lb = la;
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {  // P of 64 keys, so that PV starts while the rest is made
+          uint32_t u[64];
+          float* s = reinterpret_cast<float*>(u);
+          ptx::tmem_ld_32x32b_x32(ts + 64 * hf, u);
+          ptx::tmem_ld_32x32b_x32(ts + 64 * hf + 32, u + 32);
+          ptx::tmem_ld_wait();
+          tc_regs(u);
+          tc_regs(u + 32);
+          auto weights = [&](auto poly) {
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-          for (int c = 64 * hf; c < 64 * hf + 64; c += 2) {
-            const float p0 = tc_exp2(fmaf(s[c], mul, -mu)), p1 = tc_exp2(fmaf(s[c + 1], mul, -mu));
-            l0 += p0;
-            l1 += p1;
-            u[c >> 1] = Ty::pack(p0, p1);
+            for (int c = 0; c < 64; c += 2) {
+              float x0, x1;
+              tc_un(tc_fma2(tc_pk(s[c], s[c + 1]), mul2, mu2), x0, x1);
+              // one pair of four on the FMA pipe: the special-function pipe, 16
+              // results a cycle and SM, is the narrower one (four prompts of 4096
+              // tokens, 128-wide heads: none 597 us, 1/8 570, 1/4 561, 3/8 563;
+              // where keys are masked all on the latter, for weights of exactly 0)
+              if (decltype(poly)::value && (c & 6) == 4) {
+                tc_un(tc_poly_exp2(x0, x1), x0, x1);
+              } else {
+                x0 = tc_exp2(x0);
+                x1 = tc_exp2(x1);
+              }
+              if (c & 2) la = tc_add2(la, tc_pk(x0, x1)); else lb = tc_add2(lb, tc_pk(x0, x1));
+              u[c >> 1] = Ty::pack(x0, x1);
+            }
+          };
+          if (!back) weights(std::true_type()); else weights(std::false_type());
+          if (SEP) {
+            if (hf == 1) {       // S has been read
+              ptx::tc_fence_before();
+              tc_arrive(bar_sfree + 8 * t, lane);
+            } else if (k > 0) {  // P of the tile before has been read
+              tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
+              ptx::tc_fence_after();
+            }
           }
-          l += l0 + l1;
-          if (SEP && hf == 0 && k > 0) {  // P of the tile before has been read
-            ok = tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
-            if (!ok) break;
-            ptx::tc_fence_after();
-          }
-          ptx::tmem_st_32x32b_x32(tp + 32 * hf, u + 32 * hf);
+          ptx::tmem_st_32x32b_x32(tp + 32 * hf, u);
           ptx::tmem_st_wait();
           ptx::tc_fence_before();
           tc_arrive((hf ? bar_p2 : bar_p) + 8 * t, lane);
         }
-        if (!ok) break;
+        {
+          float l0, l1;
+          tc_un(tc_add2(la, lb), l0, l1);
+          l += l0 + l1;
+        }
       }
-      if (ok) ok = tc_wait(bar_pv + 8 * t, (uint32_t)(cnt - 1) & 1u, tmo, abort_flag);
+      tc_wait(bar_pv + 8 * t, (uint32_t)(cnt - 1) & 1u, tmo, abort_flag);
       ptx::tc_fence_after();
     }
     // ---- O / l, or the split's part of it.  Every lane takes part in the TMEM
     // loads; a half without rows, and a row behind the last, stores nothing.
-    if (half_on && ok) {
+    if (half_on) {
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: 0; NaN stays
       const int64_t prow = (int64_t)(parts.first + z) * parts.rows + (int64_t)tok * a.Hq + h;
       const bool part = parts.o != nullptr;
@@ -464,7 +568,6 @@ __global__ void __launch_bounds__(TC_NT, 1)
     const int box = lane % nb, dh = lane / nb;        // this lane's
     const int* own = a.table + (int64_t)r * a.table_stride;
     int g_ring = 0;
-    bool ok = true;
     // page number and row of this lane's box of tile k (looked up a tile ahead:
     // the table read takes as long as a tile's softmax)
     auto look = [&](int k, int& page, int& prow) {
@@ -478,16 +581,16 @@ __global__ void __launch_bounds__(TC_NT, 1)
     };
     int page, prow;
     bool mine = look(0, page, prow);
-    for (int k = 0; k < cnt && ok; ++k) {
+    for (int k = 0; k < cnt; ++k) {
       int page1, prow1;
       const bool mine1 = look(k + 1, page1, prow1);
       if (mine) mine = pg_check(a.c, page) >= 0;
       const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, mine)) * br * 128u;
 #pragma unroll
-      for (int kv = 0; kv < 2 && ok; ++kv, ++g_ring) {
+      for (int kv = 0; kv < 2; ++kv, ++g_ring) {
         const int s = g_ring % L::ST;
-        ok = tc_wait(bar_empty + 8 * s, ((uint32_t)(g_ring / L::ST) & 1u) ^ 1u, tmo, abort_flag);
-        if (!ok) break;
+        tc_wait(bar_empty + 8 * s, ((uint32_t)(g_ring / L::ST) & 1u) ^ 1u, tmo, abort_flag);
+        if (*abort_flag) break;  // (no copy into a stage that is still in use)
         if (lane == 0) ptx::mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
         __syncwarp();
         if (mine)
@@ -498,7 +601,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
       page = page1;
       prow = prow1;
     }
-    if (!ok) {  // copies in flight land before the shared memory goes
+    if (*abort_flag) {  // copies in flight land before the shared memory goes
       for (int q = g_ring > L::ST ? g_ring - L::ST : 0; q < g_ring; ++q) {
         const long long t0 = clock64();
         while (!ptx::mbar_try_wait(bar_full + 8 * (q % L::ST), (uint32_t)(q / L::ST) & 1u))
@@ -522,8 +625,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
     const uint64_t dv = ptx::smem_desc_sw128_mn(sbase + L::OFF_RING, L::HB);
     auto stage = [&](int k, int kv) { return (2 * k + kv) % L::ST; };
     auto wait_full = [&](int k, int kv) {
-      return tc_wait(bar_full + 8 * stage(k, kv), (uint32_t)((2 * k + kv) / L::ST) & 1u, tmo,
-                     abort_flag);
+      tc_wait(bar_full + 8 * stage(k, kv), (uint32_t)((2 * k + kv) / L::ST) & 1u, tmo, abort_flag);
     };
     auto qk = [&](int k, int t) {
       const uint64_t b0 = dk + (uint64_t)((stage(k, 0) * L::TILE) >> 4);
@@ -562,59 +664,43 @@ __global__ void __launch_bounds__(TC_NT, 1)
       __syncwarp();
     };
     const bool two = halves_u == 2;
-    bool ok = tc_wait(bar_q, 0, tmo, abort_flag) && wait_full(0, 0);
-    ptx::tc_fence_after();
-    if (ok) {
-      qk(0, 0);
-      if (two) qk(0, 1);
-    }
+    auto wait_p = [&](uint32_t bar, int k) {
+      tc_wait(bar, (uint32_t)k & 1u, tmo, abort_flag);
+      ptx::tc_fence_after();
+    };
+    tc_wait(bar_q, 0, tmo, abort_flag);
+    wait_full(0, 0);
+    qk(0, 0);
+    if (two) qk(0, 1);
     for (int k = 0; k < cnt_u; ++k) {
-      if (!ok) break;
       const bool more = k + 1 < cnt_u;
-      const uint32_t par = (uint32_t)k & 1u;
-      if (SEP && more) {
-        ok = wait_full(k + 1, 0) && tc_wait(bar_sfree, par, tmo, abort_flag);
-        if (!ok) break;
-        ptx::tc_fence_after();
-        qk(k + 1, 0);
-      }
-      ok = wait_full(k, 1);
-      if (!ok) break;
+      // the copies first: they are there long before P is
+      wait_full(k, 1);
       clear_tail(k);
-      ok = tc_wait(bar_p, par, tmo, abort_flag);
-      if (!ok) break;
-      ptx::tc_fence_after();
-      pv(k, 0, 0);
-      ok = tc_wait(bar_p2, par, tmo, abort_flag);
-      if (!ok) break;
-      ptx::tc_fence_after();
-      pv(k, 0, 1);
-      if (!SEP && more) {
-        ok = wait_full(k + 1, 0);
-        if (!ok) break;
-        ptx::tc_fence_after();
+      if (more) wait_full(k + 1, 0);
+      if (SEP && more) {
+        wait_p(bar_sfree, k);
         qk(k + 1, 0);
       }
+      wait_p(bar_p, k);
+      pv(k, 0, 0);
+      wait_p(bar_p2, k);
+      pv(k, 0, 1);
+      if (!SEP && more) qk(k + 1, 0);
       if (two) {
         if (SEP && more) {
-          ok = tc_wait(bar_sfree + 8, par, tmo, abort_flag);
-          if (!ok) break;
-          ptx::tc_fence_after();
+          wait_p(bar_sfree + 8, k);
           qk(k + 1, 1);
         }
-        ok = tc_wait(bar_p + 8, par, tmo, abort_flag);
-        if (!ok) break;
-        ptx::tc_fence_after();
+        wait_p(bar_p + 8, k);
         pv(k, 1, 0);
-        ok = tc_wait(bar_p2 + 8, par, tmo, abort_flag);
-        if (!ok) break;
-        ptx::tc_fence_after();
+        wait_p(bar_p2 + 8, k);
         pv(k, 1, 1);
         if (!SEP && more) qk(k + 1, 1);
       }
     }
-    if (!ok) {
-      if (lane == 0) ptx::mma_commit(bar_drain);
+    if (*abort_flag) {  // MMAs in flight end before their memory goes
+      ptx::mma_commit_if(who, bar_drain);
       const long long t0 = clock64();
       while (!ptx::mbar_try_wait(bar_drain, 0))
         if (clock64() - t0 > (long long)(tmo * 2ull)) break;
