@@ -29,7 +29,7 @@
 // rescaled: after the first tiles a row's maximum hardly grows.
 //
 // Warps 0-3 and 4-7: softmax of half 0 and 1.  Warp 8: TMA, one box per page
-// and 64 dimensions, each lane its own.  Warp 9: MMA issue.  While one half is
+// and 64 dimensions, each lane its own.  Warps 9 and 10: MMA issue, a half each.  While one half is
 // in its softmax the tensor core works for the other.  64-wide heads leave TMEM
 // for P beside S, so S of the next tile is made during the softmax of this one;
 // with 128-wide heads P takes S's place and it follows PV.
@@ -62,9 +62,11 @@ struct TcLayout {
   static constexpr int OFF_RING = 2 * TILE;
   static constexpr int OFF_BAR = OFF_RING + ST * TILE;
   static constexpr int SMEM = OFF_BAR + 512 + 1024;
-  static constexpr bool SEP = D == 64;           // P beside S
-  static constexpr int COL_S = 0, COL_P = SEP ? 256 : 0, STEP_P = SEP ? 64 : 128;
-  static constexpr int COL_O = SEP ? 384 : 256;
+  // TMEM columns: scores (64-wide heads: of each half; 128-wide ones: of both in
+  // turn), weights and outputs of each half
+  static constexpr bool ONE_S = D == 128;
+  static constexpr int COL_S = 0, STEP_S = ONE_S ? 0 : 128;
+  static constexpr int COL_P = ONE_S ? 128 : 256, COL_O = COL_P + 128;
 };
 
 __device__ __forceinline__ float tc_exp2(float x) {
@@ -142,18 +144,19 @@ __device__ __forceinline__ TcF2 tc_poly_exp2(float x0, float x1) {
 // buffers hold, and no lane leaves its warp in between.  A wait on a phase that
 // is complete costs 55 cycles this way; with an answer for the warp to branch on
 // it cost 106, six times per pair of tiles on the path from P to the next S.
-__device__ __forceinline__ void tc_wait_slow(uint32_t bar, uint32_t parity, uint64_t tmo,
-                                          volatile int* abort) {
-  const long long t0 = clock64();
-  while (!*abort) {
-    for (int n = 0; n < 64; ++n)
-      if (ptx::mbar_try_wait_now(bar, parity)) return;
-    if (clock64() - t0 > (long long)(tmo * 2ull)) *abort = 1;
-  }
-}
-__device__ __forceinline__ void tc_wait(uint32_t bar, uint32_t parity, uint64_t tmo,
+// (Short on purpose: the warps of a quarter of the SM share a small instruction
+// cache.  The limit is in polls of at least 50 cycles, so a wait at lower clocks
+// only lasts longer.)
+__device__ __forceinline__ void tc_wait(uint32_t bar, uint32_t parity, uint32_t polls,
                                         volatile int* abort) {
-  if (!ptx::mbar_try_wait_now(bar, parity)) tc_wait_slow(bar, parity, tmo, abort);
+  if (!ptx::mbar_try_wait_now(bar, parity)) {
+    while (!ptx::mbar_try_wait(bar, parity)) {
+      if (*abort || --polls == 0) {
+        *abort = 1;
+        break;
+      }
+    }
+  }
   __syncwarp();
 }
 
@@ -176,12 +179,13 @@ __global__ void __launch_bounds__(TC_NT, 1)
                     const PgParts parts, const int splits, const unsigned long long tmo) {
   using L = TcLayout<D>;
   using Ty = PgType<E>;
-  constexpr bool SEP = L::SEP;
+  constexpr bool ONE_S = L::ONE_S;
   extern __shared__ uint8_t tc_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   const uint32_t sbase = ptx::smem_u32(smem);
   __shared__ int found[6], wsum[TC_NT / 32];  // request, tile, first row, rows, keys, bidir
+  const uint32_t polls = (uint32_t)min(tmo / 25ull + 1ull, 0xffffffffull);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.Hq / a.c.Hkv, g = blockIdx.y, z = blockIdx.z;
 
@@ -189,17 +193,17 @@ __global__ void __launch_bounds__(TC_NT, 1)
   const uint32_t bar_empty = bar_full + 8 * L::ST;
   const uint32_t bar_q = bar_empty + 8 * L::ST;
   const uint32_t bar_s = bar_q + 8;         // [2] scores ready
-  const uint32_t bar_sfree = bar_s + 16;    // [2] scores read (SEP)
+  const uint32_t bar_sfree = bar_s + 16;    // [2] scores read
   const uint32_t bar_p = bar_sfree + 16;    // [2] weights ready
   const uint32_t bar_p2 = bar_p + 16;       // [2] ... of the tile's second 64 keys
   const uint32_t bar_pv = bar_p2 + 16;      // [2] PV done
   const uint32_t bar_drain = bar_pv + 16;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_BAR + 8 * (2 * L::ST + 12));
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_BAR + 8 * (2 * L::ST + 13));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   if (tid == 0) {
     for (int s = 0; s < L::ST; ++s) {
       ptx::mbar_init(bar_full + 8 * s, 1);
-      ptx::mbar_init(bar_empty + 8 * s, 1);
+      ptx::mbar_init(bar_empty + 8 * s, 2);  // the MMAs of both halves
     }
     ptx::mbar_init(bar_q, 8);  // warps
     for (int t = 0; t < 2; ++t) {
@@ -210,6 +214,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
       ptx::mbar_init(bar_pv + 8 * t, 1);
     }
     ptx::mbar_init(bar_drain, 1);
+    ptx::mbar_init(bar_drain + 8, 1);
     *abort_flag = 0;
     found[0] = -1;
     ptx::fence_mbar_init();
@@ -355,8 +360,8 @@ __global__ void __launch_bounds__(TC_NT, 1)
       tc_arrive(bar_q, lane);
     }
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + L::COL_S + t * 128 + lanes;
-    const uint32_t tp = tmem + L::COL_P + t * L::STEP_P + lanes;
+    const uint32_t ts = tmem + L::COL_S + t * L::STEP_S + lanes;
+    const uint32_t tp = tmem + L::COL_P + t * 64 + lanes;
     const uint32_t to = tmem + L::COL_O + t * D + lanes;
     if (half_on) {
       constexpr float LOG2E = 1.4426950408889634f;
@@ -367,71 +372,53 @@ __global__ void __launch_bounds__(TC_NT, 1)
         const int j0 = key0(k);
         const int lim = min(end, limit(k)) - j0;  // keys of this tile that the row attends
         const bool full = __all_sync(0xffffffffu, lim >= TC_KV);
-        tc_wait(bar_s + 8 * t, (uint32_t)k & 1u, tmo, abort_flag);
-        // (P in S's place: the PV of the tile before is done too, as its MMAs
-        // were issued before those of S; its barrier is waited for here so that
-        // no phase of it is skipped)
-        if (!SEP && k > 0) tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
+        tc_wait(bar_s + 8 * t, (uint32_t)k & 1u, polls, abort_flag);
         ptx::tc_fence_after();
-        // The row passes through registers 64 scores at a time, twice (a TMEM load
-        // of 64 columns takes 25 cycles): once for the maximum, once for the
-        // weights.  Loops, not 128 scores unrolled: the code of a tile in
-        // straight lines (16 KB a variant) kept the instruction caches busy, and
-        // the MMA warp waited hundreds of cycles for its next instruction.
-        const bool back = !plain || !full;  // scores changed on the way: put back
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t u[64];
-          float* s = reinterpret_cast<float*>(u);
-          ptx::tmem_ld_32x32b_x32(ts + 64 * hf, u);
-          ptx::tmem_ld_32x32b_x32(ts + 64 * hf + 32, u + 32);
-          ptx::tmem_ld_wait();
-          tc_regs(u);
-          tc_regs(u + 32);
-          if (back) {
-            if (!plain) {  // to log2 units, capped and biased
-              if (a.cap > 0.f) {
-                // cap tanh(y / cap) = cap - 2 cap / (exp(2 y / cap) + 1): an absolute
-                // error of a few 2^-23 cap, also where the exponential overflows
-                const float kk = 2.f * LOG2E * a.scale / a.cap, A = a.cap * LOG2E;
+        // the row into registers, and S is free for the next scores
+        uint32_t u[128];
+        float* s = reinterpret_cast<float*>(u);
 #pragma unroll
-                for (int c = 0; c < 64; ++c)
-                  s[c] = fmaf(-2.f * A, tc_rcp(tc_exp2(s[c] * kk) + 1.f), A);
-              } else {
-                const float kk = a.scale * LOG2E;
+        for (int c = 0; c < 128; c += 32) ptx::tmem_ld_32x32b_x32(ts + c, u + c);
+        ptx::tmem_ld_wait();
 #pragma unroll
-                for (int c = 0; c < 64; ++c) s[c] *= kk;
-              }
-              if (a.slopes) {
-                const float d0 = (float)(pos - j0 - 64 * hf);
+        for (int c = 0; c < 128; c += 32) tc_regs(u + c);
+        ptx::tc_fence_before();
+        tc_arrive(bar_sfree + 8 * t, lane);
+        if (!plain) {  // to log2 units, capped and biased
+          if (a.cap > 0.f) {
+            // cap tanh(y / cap) = cap - 2 cap / (exp(2 y / cap) + 1): an absolute
+            // error of a few 2^-23 cap, also where the exponential overflows
+            const float kk = 2.f * LOG2E * a.scale / a.cap, A = a.cap * LOG2E;
 #pragma unroll
-                for (int c = 0; c < 64; ++c) s[c] = fmaf(-slope, fabsf(d0 - (float)c), s[c]);
-              }
-            }
-            if (!full) {
-              const int lh = lim - 64 * hf;
+            for (int c = 0; c < 128; ++c)
+              s[c] = fmaf(-2.f * A, tc_rcp(tc_exp2(s[c] * kk) + 1.f), A);
+          } else {
+            const float kk = a.scale * LOG2E;
 #pragma unroll
-              for (int c = 0; c < 64; ++c)
-                if (c >= lh) s[c] = -INFINITY;
-            }
-            ptx::tmem_st_32x32b_x32(ts + 64 * hf, u);
-            ptx::tmem_st_32x32b_x32(ts + 64 * hf + 32, u + 32);
+            for (int c = 0; c < 128; ++c) s[c] *= kk;
           }
-          float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
+          if (a.slopes) {
+            const float d0 = (float)(pos - j0);
 #pragma unroll
-          for (int c = 4; c < 60; c += 8) {
-            x0 = tc_max3(x0, s[c], s[c + 1]);
-            x1 = tc_max3(x1, s[c + 2], s[c + 3]);
-            x2 = tc_max3(x2, s[c + 4], s[c + 5]);
-            x3 = tc_max3(x3, s[c + 6], s[c + 7]);
+            for (int c = 0; c < 128; ++c) s[c] = fmaf(-slope, fabsf(d0 - (float)c), s[c]);
           }
-          x0 = tc_max3(x0, s[60], s[61]);
-          x1 = tc_max3(x1, s[62], s[63]);
-          mx = tc_max3(mx, fmaxf(x0, x1), fmaxf(x2, x3));
         }
-        if (back) ptx::tmem_st_wait();
-        mx *= mul;
+        if (!full) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c >= lim) s[c] = -INFINITY;
+        }
+        float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
+#pragma unroll
+        for (int c = 4; c < 124; c += 8) {
+          x0 = tc_max3(x0, s[c], s[c + 1]);
+          x1 = tc_max3(x1, s[c + 2], s[c + 3]);
+          x2 = tc_max3(x2, s[c + 4], s[c + 5]);
+          x3 = tc_max3(x3, s[c + 6], s[c + 7]);
+        }
+        x0 = tc_max3(x0, s[124], s[125]);
+        x1 = tc_max3(x1, s[126], s[127]);
+        const float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * mul;
         if (__any_sync(0xffffffffu, mx > m + TC_LAZY)) {
           float alpha = 1.f;
           if (mx > m + TC_LAZY) {  // also the first keys of the row (m = -inf)
@@ -440,64 +427,53 @@ __global__ void __launch_bounds__(TC_NT, 1)
             l *= alpha;
           }
           if (k > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            if constexpr (SEP) {
-              tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
-              ptx::tc_fence_after();
-            }
-#pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              ptx::tmem_ld_32x32b_x32(to + c, o);
+            tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, polls, abort_flag);
+            ptx::tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              ptx::tmem_ld_32x32b_x16(to + c, o);
               ptx::tmem_ld_wait();
-              tc_regs(o);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              ptx::tmem_st_32x32b_x32(to + c, o);
+              for (int e = 0; e < 16; e += 4)
+                asm volatile("" : "+r"(o[e]), "+r"(o[e + 1]), "+r"(o[e + 2]), "+r"(o[e + 3]));
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              ptx::tmem_st_32x32b_x16(to + c, o);
             }
           }
         }
         const float mu = m == -INFINITY ? 0.f : m;
         const TcF2 mul2 = tc_pk(mul, mul), mu2 = tc_pk(-mu, -mu);
         TcF2 la = tc_pk(0.f, 0.f), lb = la;
-#pragma unroll 1
-        for (int hf = 0; hf < 2; ++hf) {  // P of 64 keys, so that PV starts while the rest is made
-          uint32_t u[64];
-          float* s = reinterpret_cast<float*>(u);
-          ptx::tmem_ld_32x32b_x32(ts + 64 * hf, u);
-          ptx::tmem_ld_32x32b_x32(ts + 64 * hf + 32, u + 32);
-          ptx::tmem_ld_wait();
-          tc_regs(u);
-          tc_regs(u + 32);
-          auto weights = [&](auto poly) {
+        // P of 64 keys at a time, so that PV starts while the rest is made
+        auto weights = [&](int hf, auto poly) {
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) {
-              float x0, x1;
-              tc_un(tc_fma2(tc_pk(s[c], s[c + 1]), mul2, mu2), x0, x1);
-              // one pair of four on the FMA pipe: the special-function pipe, 16
-              // results a cycle and SM, is the narrower one (four prompts of 4096
-              // tokens, 128-wide heads: none 597 us, 1/8 570, 1/4 561, 3/8 563;
-              // where keys are masked all on the latter, for weights of exactly 0)
-              if (decltype(poly)::value && (c & 6) == 4) {
-                tc_un(tc_poly_exp2(x0, x1), x0, x1);
-              } else {
-                x0 = tc_exp2(x0);
-                x1 = tc_exp2(x1);
-              }
-              if (c & 2) la = tc_add2(la, tc_pk(x0, x1)); else lb = tc_add2(lb, tc_pk(x0, x1));
-              u[c >> 1] = Ty::pack(x0, x1);
+          for (int c = 64 * hf; c < 64 * hf + 64; c += 2) {
+            float y0, y1;
+            tc_un(tc_fma2(tc_pk(s[c], s[c + 1]), mul2, mu2), y0, y1);
+            // one pair of four on the FMA pipe: the special-function pipe, 16
+            // results a cycle and SM, is the narrower one (four prompts of 4096
+            // tokens, 128-wide heads: none 597 us, 1/8 570, 1/4 561, 3/8 563;
+            // where keys are masked all on the latter, for weights of exactly 0)
+            if (decltype(poly)::value && (c & 6) == 4) {
+              tc_un(tc_poly_exp2(y0, y1), y0, y1);
+            } else {
+              y0 = tc_exp2(y0);
+              y1 = tc_exp2(y1);
             }
-          };
-          if (!back) weights(std::true_type()); else weights(std::false_type());
-          if (SEP) {
-            if (hf == 1) {       // S has been read
-              ptx::tc_fence_before();
-              tc_arrive(bar_sfree + 8 * t, lane);
-            } else if (k > 0) {  // P of the tile before has been read
-              tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
-              ptx::tc_fence_after();
-            }
+            if (c & 2) la = tc_add2(la, tc_pk(y0, y1)); else lb = tc_add2(lb, tc_pk(y0, y1));
+            u[c >> 1] = Ty::pack(y0, y1);
           }
-          ptx::tmem_st_32x32b_x32(tp + 32 * hf, u);
+        };
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          if (full) weights(hf, std::true_type()); else weights(hf, std::false_type());
+          if (hf == 0 && k > 0) {  // P of the tile before has been read
+            tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, polls, abort_flag);
+            ptx::tc_fence_after();
+          }
+          ptx::tmem_st_32x32b_x32(tp + 32 * hf, u + 32 * hf);
           ptx::tmem_st_wait();
           ptx::tc_fence_before();
           tc_arrive((hf ? bar_p2 : bar_p) + 8 * t, lane);
@@ -508,7 +484,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
           l += l0 + l1;
         }
       }
-      tc_wait(bar_pv + 8 * t, (uint32_t)(cnt - 1) & 1u, tmo, abort_flag);
+      tc_wait(bar_pv + 8 * t, (uint32_t)(cnt - 1) & 1u, polls, abort_flag);
       ptx::tc_fence_after();
     }
     // ---- O / l, or the split's part of it.  Every lane takes part in the TMEM
@@ -589,7 +565,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv, ++g_ring) {
         const int s = g_ring % L::ST;
-        tc_wait(bar_empty + 8 * s, ((uint32_t)(g_ring / L::ST) & 1u) ^ 1u, tmo, abort_flag);
+        tc_wait(bar_empty + 8 * s, ((uint32_t)(g_ring / L::ST) & 1u) ^ 1u, polls, abort_flag);
         if (*abort_flag) break;  // (no copy into a stage that is still in use)
         if (lane == 0) ptx::mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
         __syncwarp();
@@ -608,101 +584,117 @@ __global__ void __launch_bounds__(TC_NT, 1)
           if (clock64() - t0 > (long long)(tmo * 2ull)) break;
       }
     }
-    } else if (warp == 9) {
+    } else if (warp - 9 < halves) {
     // -------------------------------------------------------------------- MMA
+    // One warp per half: an iteration's waits, descriptors and MMAs are some
+    // hundred dependent instructions, which one warp for both halves did not get
+    // through in the time of a softmax (2900 cycles a pair of tiles, whatever the
+    // softmax took).  Uniform copies: the loop and every operand of its MMAs are
+    // the same for the warp, and the compiler can see it (an MMA whose
+    // descriptors come from vector registers took 130 cycles to issue).
     constexpr bool BF = sizeof(E) == 2 && !std::is_same<E, __half>::value;
     constexpr uint32_t id_qk = ptx::idesc_16_f32(TC_HALF, TC_KV, BF, false);
     constexpr uint32_t id_pv = ptx::idesc_16_f32(TC_HALF, D, BF, true);
-    // uniform copies: the loop below and every operand of its MMAs are the same
-    // for the warp, and the compiler can see it (an MMA whose descriptors come
-    // from vector registers took 130 cycles to issue)
+    const int t = __reduce_max_sync(0xffffffffu, warp - 9);
     const int cnt_u = __reduce_max_sync(0xffffffffu, cnt);
     const int halves_u = __reduce_max_sync(0xffffffffu, halves);
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
     const uint32_t who = ptx::elect_one();
-    const uint64_t dq = ptx::smem_desc_sw128(sbase);
+    const uint64_t dq = ptx::smem_desc_sw128(sbase + t * L::TILE);
     const uint64_t dk = ptx::smem_desc_sw128(sbase + L::OFF_RING);
     const uint64_t dv = ptx::smem_desc_sw128_mn(sbase + L::OFF_RING, L::HB);
-    auto stage = [&](int k, int kv) { return (2 * k + kv) % L::ST; };
-    auto wait_full = [&](int k, int kv) {
-      tc_wait(bar_full + 8 * stage(k, kv), (uint32_t)((2 * k + kv) / L::ST) & 1u, tmo, abort_flag);
-    };
-    auto qk = [&](int k, int t) {
-      const uint64_t b0 = dk + (uint64_t)((stage(k, 0) * L::TILE) >> 4);
-      const uint64_t a0 = dq + (uint64_t)((t * L::TILE) >> 4);
-#pragma unroll
-      for (int e = 0; e < D / 16; ++e) {
-        const uint64_t o = (uint64_t)(((e >> 2) * L::HB + (e & 3) * 32) >> 4);
-        ptx::mma_f16_ss_if(who, tm + L::COL_S + t * 128, a0 + o, b0 + o, id_qk,
-                           e != 0 ? 1u : 0u);
-      }
-      ptx::mma_commit_if(who, bar_s + 8 * t);
-      if (t == halves_u - 1) ptx::mma_commit_if(who, bar_empty + 8 * stage(k, 0));
-    };
-    auto pv = [&](int k, int t, int hf) {  // 64 keys
-      const uint64_t b0 = dv + (uint64_t)((stage(k, 1) * L::TILE) >> 4);
-      const uint32_t p0 = tm + L::COL_P + t * L::STEP_P;
-#pragma unroll
-      for (int e = 4 * hf; e < 4 * hf + 4; ++e)
-        ptx::mma_f16_ts_if(who, tm + L::COL_O + t * D, p0 + e * 8,
-                           b0 + (uint64_t)((e * 2048) >> 4), id_pv, (k | e) != 0 ? 1u : 0u);
-      if (hf == 0) return;
-      ptx::mma_commit_if(who, bar_pv + 8 * t);
-      if (t == halves_u - 1) ptx::mma_commit_if(who, bar_empty + 8 * stage(k, 1));
-    };
-    // V's rows behind the last key may hold anything (or were not loaded): their
-    // weights are zero, and 0 x NaN is NaN
-    auto clear_tail = [&](int k) {
-      const int have = limit(k) - key0(k);
-      if (have >= TC_KV) return;
-      uint8_t* vs = smem + L::OFF_RING + stage(k, 1) * L::TILE;
-      for (int x = have * 8 + lane; x < TC_KV * 8; x += 32)
-#pragma unroll
-        for (int hb = 0; hb < D / 64; ++hb)
-          *reinterpret_cast<uint4*>(vs + hb * L::HB + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-    };
-    const bool two = halves_u == 2;
-    auto wait_p = [&](uint32_t bar, int k) {
-      tc_wait(bar, (uint32_t)k & 1u, tmo, abort_flag);
-      ptx::tc_fence_after();
-    };
-    tc_wait(bar_q, 0, tmo, abort_flag);
-    wait_full(0, 0);
-    qk(0, 0);
-    if (two) qk(0, 1);
-    for (int k = 0; k < cnt_u; ++k) {
-      const bool more = k + 1 < cnt_u;
-      // the copies first: they are there long before P is
-      wait_full(k, 1);
-      clear_tail(k);
-      if (more) wait_full(k + 1, 0);
-      if (SEP && more) {
-        wait_p(bar_sfree, k);
-        qk(k + 1, 0);
-      }
-      wait_p(bar_p, k);
-      pv(k, 0, 0);
-      wait_p(bar_p2, k);
-      pv(k, 0, 1);
-      if (!SEP && more) qk(k + 1, 0);
-      if (two) {
-        if (SEP && more) {
-          wait_p(bar_sfree + 8, k);
-          qk(k + 1, 1);
+    const uint32_t tm_s = tm + L::COL_S + t * L::STEP_S, tm_p = tm + L::COL_P + t * 64,
+                   tm_o = tm + L::COL_O + t * D;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      uint32_t n = polls;
+      while (!ptx::mbar_try_wait_now(bar, parity)) {
+        if (*abort_flag || --n == 0) {
+          *abort_flag = 1;
+          break;
         }
-        wait_p(bar_p + 8, k);
-        pv(k, 1, 0);
-        wait_p(bar_p2 + 8, k);
-        pv(k, 1, 1);
-        if (!SEP && more) qk(k + 1, 1);
+      }
+    };
+    // the stage is free when both halves are done with it: the only half says so
+    // twice
+    auto release = [&](int s) {
+      ptx::mma_commit_if(who, bar_empty + 8 * s);
+      if (halves_u == 1) ptx::mma_commit_if(who, bar_empty + 8 * s);
+    };
+    auto qk = [&](int s) {  // K in stage s
+      const uint64_t b0 = dk + (uint64_t)(s * (L::TILE >> 4));
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e)
+        ptx::mma_f16_ss_if(who, tm_s, dq + ((e >> 2) * L::HB + (e & 3) * 32) / 16,
+                           b0 + ((e >> 2) * L::HB + (e & 3) * 32) / 16, id_qk, e != 0 ? 1u : 0u);
+      ptx::mma_commit_if(who, bar_s + 8 * t);
+      release(s);
+    };
+    wait(bar_q, 0);
+    wait(bar_full, 0);
+    // half 1's first scores go where half 0's were, once those have been read
+    if (ONE_S && t == 1) {
+      wait(bar_sfree, 0);
+      ptx::tc_fence_after();
+    }
+    qk(0);
+    int sk = 2 % L::ST, sv = 1;       // stages of K of the next tile and V of this one
+    uint32_t phk = 0, phv = 0, par = 0;
+#pragma unroll 1
+    for (int k = 0; k < cnt_u; ++k, par ^= 1u) {
+      wait(bar_full + 8 * sv, phv);
+      const int have = limit(k) - key0(k);
+      if (have < TC_KV) {
+        // V's rows behind the last key may hold anything (or were not loaded):
+        // their weights are zero, and 0 x NaN is NaN.  (Both halves' warps write
+        // the zeros, each before its own MMAs.)
+        uint8_t* vs = smem + L::OFF_RING + sv * L::TILE;
+        for (int x = have * 8 + lane; x < TC_KV * 8; x += 32)
+#pragma unroll
+          for (int hb = 0; hb < D / 64; ++hb)
+            *reinterpret_cast<uint4*>(vs + hb * L::HB + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (k + 1 < cnt_u) {
+        wait(bar_full + 8 * sk, phk);
+        // S is free once it has been read: by its own half, or, where both share
+        // it, by the other one (half 1 of this tile; half 0 of the next)
+        if (ONE_S && halves_u == 2)
+          wait(bar_sfree + 8 * (1 - t), t == 0 ? par : par ^ 1u);
+        else
+          wait(bar_sfree + 8 * t, par);
+        ptx::tc_fence_after();
+        qk(sk);
+      }
+      const uint64_t b0 = dv + (uint64_t)(sv * (L::TILE >> 4));
+      wait(bar_p + 8 * t, par);
+      ptx::tc_fence_after();
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        ptx::mma_f16_ts_if(who, tm_o, tm_p + e * 8, b0 + e * 128, id_pv, (k | e) != 0 ? 1u : 0u);
+      wait(bar_p2 + 8 * t, par);
+      ptx::tc_fence_after();
+#pragma unroll
+      for (int e = 4; e < 8; ++e)
+        ptx::mma_f16_ts_if(who, tm_o, tm_p + e * 8, b0 + e * 128, id_pv, 1u);
+      ptx::mma_commit_if(who, bar_pv + 8 * t);
+      release(sv);
+      sk += 2;
+      if (sk >= L::ST) {
+        sk -= L::ST;
+        phk ^= 1u;
+      }
+      sv += 2;
+      if (sv >= L::ST) {
+        sv -= L::ST;
+        phv ^= 1u;
       }
     }
+    __syncwarp();
     if (*abort_flag) {  // MMAs in flight end before their memory goes
-      ptx::mma_commit_if(who, bar_drain);
+      ptx::mma_commit_if(who, bar_drain + 8 * t);
       const long long t0 = clock64();
-      while (!ptx::mbar_try_wait(bar_drain, 0))
+      while (!ptx::mbar_try_wait(bar_drain + 8 * t, 0))
         if (clock64() - t0 > (long long)(tmo * 2ull)) break;
     }
     }
