@@ -251,6 +251,23 @@ __global__ void __launch_bounds__(DC_NW * 32)
   const float mul = plain ? a.scale * LOG2E : 1.f;
   uint32_t q[NB][D / 16][2];
   float m[NB][2], l[NB][2], slope[NB][2], o[D / 16][NB][4];
+  // the queries of a segment, requested while the segment before it is joined
+  auto load_q = [&](const DcWalk& w) {
+    const int grp = w.seg % groups, heads = min(16, G - grp * 16);
+    const E* base = reinterpret_cast<const E*>(a.q) + w.b * a.q_ts + col2;
+    const int first = w.seg / groups * G + grp * 16;
+#pragma unroll
+    for (int nbk = 0; nbk < NB; ++nbk) {
+      const int hq = row4 + 8 * nbk;
+      const E* src = base + (int64_t)(first + hq) * a.q_hs;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) {
+        q[nbk][e][0] = hq < heads ? *reinterpret_cast<const uint32_t*>(src + 16 * e) : 0u;
+        q[nbk][e][1] = hq < heads ? *reinterpret_cast<const uint32_t*>(src + 16 * e + 8) : 0u;
+      }
+    }
+  };
+  load_q(cw);
   bool fresh = true;      // the next unit starts a part of a segment
   bool whole = true;      // ... which begins in this CTA
   int used = 0;
@@ -263,14 +280,6 @@ __global__ void __launch_bounds__(DC_NW * 32)
       whole = cw.c == 0;
 #pragma unroll
       for (int nbk = 0; nbk < NB; ++nbk) {
-        const int hq = row4 + 8 * nbk;
-        const E* src = reinterpret_cast<const E*>(a.q) + cw.b * a.q_ts +
-                       (int64_t)(h0 + hq) * a.q_hs + col2;
-#pragma unroll
-        for (int e = 0; e < D / 16; ++e) {
-          q[nbk][e][0] = hq < heads ? *reinterpret_cast<const uint32_t*>(src + 16 * e) : 0u;
-          q[nbk][e][1] = hq < heads ? *reinterpret_cast<const uint32_t*>(src + 16 * e + 8) : 0u;
-        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           m[nbk][x] = -INFINITY;
@@ -409,6 +418,7 @@ __global__ void __launch_bounds__(DC_NW * 32)
     if (cw.c != 0 && u + 1 < count) continue;
     // ---- the end of this CTA's part of the segment: the warps' results, joined
     fresh = true;
+    if (u + 1 < count) load_q(cw);
 #pragma unroll
     for (int nbk = 0; nbk < NB; ++nbk)
 #pragma unroll
@@ -519,19 +529,31 @@ __global__ void __launch_bounds__(256)
   for (int z0 = 0; z0 < n; z0 += 32) {
     const float ls = lse_of(z0 + lane);
     const float wl = ls == -INFINITY ? 0.f : exp2f(ls - mx);
-    for (int z = 0; z < min(32, n - z0); ++z) {
-      const float w = __shfl_sync(0xffffffffu, wl, z);
-      if (w == 0.f) continue;
-      const float* src = (z0 + z < first ? p.o + ((z0 + z) * p.rows + row) * D
-                                         : side.o + index(z0 + z) * D) + lane * DPL;
-      float v[DPL];
-      if constexpr (DPL == 2)
-        *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
-      else
-        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-      den += w;
+    const int m = min(32, n - z0);
+    for (int z1 = 0; z1 < m; z1 += 4) {  // four parts in flight
+      float v[4][DPL], w[4];
 #pragma unroll
-      for (int e = 0; e < DPL; ++e) o[e] = fmaf(w, v[e], o[e]);
+      for (int y = 0; y < 4; ++y) {
+        const int z = z0 + z1 + y;
+        w[y] = __shfl_sync(0xffffffffu, wl, (z1 + y) & 31);
+        if (z >= n) w[y] = 0.f;
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) v[y][e] = 0.f;
+        if (w[y] != 0.f) {  // a part without keys was not written
+          const float* src =
+              (z < first ? p.o + (z * p.rows + row) * D : side.o + index(z) * D) + lane * DPL;
+          if constexpr (DPL == 2)
+            *reinterpret_cast<float2*>(v[y]) = *reinterpret_cast<const float2*>(src);
+          else
+            *reinterpret_cast<float4*>(v[y]) = *reinterpret_cast<const float4*>(src);
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        den += w[y];
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) o[e] = fmaf(w[y], v[y][e], o[e]);
+      }
     }
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;  // NaN stays NaN

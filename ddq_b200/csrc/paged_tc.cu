@@ -386,12 +386,36 @@ __global__ void __launch_bounds__(TC_NT, 1)
         tc_arrive(bar_sfree + 8 * t, lane);
         if (!plain) {  // to log2 units, capped and biased
           if (a.cap > 0.f) {
-            // cap tanh(y / cap) = cap - 2 cap / (exp(2 y / cap) + 1): an absolute
-            // error of a few 2^-23 cap, also where the exponential overflows
-            const float kk = 2.f * LOG2E * a.scale / a.cap, A = a.cap * LOG2E;
+            float big = 0.f;
 #pragma unroll
-            for (int c = 0; c < 128; ++c)
-              s[c] = fmaf(-2.f * A, tc_rcp(tc_exp2(s[c] * kk) + 1.f), A);
+            for (int c = 0; c < 128; c += 2) big = tc_max3(big, fabsf(s[c]), fabsf(s[c + 1]));
+            if (__all_sync(0xffffffffu, big * fabsf(a.scale) <= 0.5f * a.cap)) {
+              // |y| <= 1/2, y = scale s / cap: cap tanh(y) = scale s P(y^2), P the
+              // minimax polynomial of degree 4 of tanh(sqrt u) / sqrt(u) on [0, 1/4]
+              // (Remez, error 2^-26), its coefficients in powers of s^2: six packed
+              // operations for two scores, no special function
+              const float kk = a.scale * LOG2E, r2 = (a.scale / a.cap) * (a.scale / a.cap);
+              const float cap0 = kk * 0.999999987f, cap1 = kk * -0.333330694f * r2,
+                          cap2 = kk * 0.133247793f * (r2 * r2),
+                          cap3 = kk * -0.0529860753f * (r2 * r2 * r2),
+                          cap4 = kk * 0.0171350066f * (r2 * r2) * (r2 * r2);
+#pragma unroll
+              for (int c = 0; c < 128; c += 2) {
+                const TcF2 x = tc_pk(s[c], s[c + 1]), v = tc_mul2(x, x);
+                TcF2 q = tc_fma2(v, tc_pk(cap4, cap4), tc_pk(cap3, cap3));
+                q = tc_fma2(v, q, tc_pk(cap2, cap2));
+                q = tc_fma2(v, q, tc_pk(cap1, cap1));
+                q = tc_fma2(v, q, tc_pk(cap0, cap0));
+                tc_un(tc_mul2(x, q), s[c], s[c + 1]);
+              }
+            } else {
+              // cap tanh(y) = cap - 2 cap / (exp(2 y) + 1): an absolute error of a
+              // few 2^-23 cap, also where the exponential overflows
+              const float kk = 2.f * LOG2E * a.scale / a.cap, A = a.cap * LOG2E;
+#pragma unroll
+              for (int c = 0; c < 128; ++c)
+                s[c] = fmaf(-2.f * A, tc_rcp(tc_exp2(s[c] * kk) + 1.f), A);
+            }
           } else {
             const float kk = a.scale * LOG2E;
 #pragma unroll
@@ -399,8 +423,16 @@ __global__ void __launch_bounds__(TC_NT, 1)
           }
           if (a.slopes) {
             const float d0 = (float)(pos - j0);
+            const TcF2 d2 = tc_pk(d0, d0), sl2 = tc_pk(-slope, -slope);
+            if (__all_sync(0xffffffffu, pos - j0 >= TC_KV - 1)) {  // no key behind the row
 #pragma unroll
-            for (int c = 0; c < 128; ++c) s[c] = fmaf(-slope, fabsf(d0 - (float)c), s[c]);
+              for (int c = 0; c < 128; c += 2)
+                tc_un(tc_fma2(sl2, tc_add2(d2, tc_pk((float)-c, (float)(-c - 1))),
+                              tc_pk(s[c], s[c + 1])), s[c], s[c + 1]);
+            } else {
+#pragma unroll
+              for (int c = 0; c < 128; ++c) s[c] = fmaf(-slope, fabsf(d0 - (float)c), s[c]);
+            }
           }
         }
         if (!full) {
@@ -468,7 +500,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
         };
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          if (full) weights(hf, std::true_type()); else weights(hf, std::false_type());
+          if (full && plain) weights(hf, std::true_type()); else weights(hf, std::false_type());
           if (hf == 0 && k > 0) {  // P of the tile before has been read
             tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, polls, abort_flag);
             ptx::tc_fence_after();
@@ -730,18 +762,29 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PgAttnArgs a, co
   for (int z0 = 0; z0 < p.count; z0 += 32) {
     const float ls = z0 + lane < p.count ? p.lse[(z0 + lane) * p.rows + row] : -INFINITY;
     const float wl = ls == -INFINITY ? 0.f : exp2f(ls - mx);
-    for (int z = 0; z < min(32, p.count - z0); ++z) {
-      const float w = __shfl_sync(0xffffffffu, wl, z);
-      if (w == 0.f) continue;
-      const float* src = p.o + ((z0 + z) * p.rows + row) * D + lane * DPL;
-      float v[DPL];
-      if constexpr (DPL == 2)
-        *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
-      else
-        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-      den += w;
+    const int m = min(32, p.count - z0);
+    for (int z1 = 0; z1 < m; z1 += 4) {  // four parts in flight
+      float v[4][DPL], w[4];
 #pragma unroll
-      for (int e = 0; e < DPL; ++e) o[e] = fmaf(w, v[e], o[e]);
+      for (int y = 0; y < 4; ++y) {
+        w[y] = __shfl_sync(0xffffffffu, wl, (z1 + y) & 31);
+        if (z1 + y >= m) w[y] = 0.f;
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) v[y][e] = 0.f;
+        if (w[y] != 0.f) {  // a part without keys was not written
+          const float* src = p.o + ((z0 + z1 + y) * p.rows + row) * D + lane * DPL;
+          if constexpr (DPL == 2)
+            *reinterpret_cast<float2*>(v[y]) = *reinterpret_cast<const float2*>(src);
+          else
+            *reinterpret_cast<float4*>(v[y]) = *reinterpret_cast<const float4*>(src);
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        den += w[y];
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) o[e] = fmaf(w[y], v[y][e], o[e]);
+      }
     }
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;  // NaN stays NaN
