@@ -4,18 +4,19 @@
 //
 // HBM bound: every key and value is read once for the heads that share it, and
 // sequences differ in length by orders of magnitude.  So the work is a flat
-// list of units of 128 keys - sequence, key/value head (and group of 16 query
-// heads), unit of the sequence - which the CTAs, as many as fit the GPU, share
-// out evenly: CTA i of N takes units [i U / N, (i + 1) U / N), whatever
+// list of units of 32 keys - sequence, key/value head (and group of 16 query
+// heads), unit of the sequence - which the warps of as many CTAs as fit the GPU
+// share out evenly: warp i of N takes units [i U / N, (i + 1) U / N), whatever
 // sequences they belong to.  The list is never stored: each CTA sums the
-// lengths (4 bytes a sequence) and finds its first unit.  Where a CTA's range
-// cuts a sequence, its part goes to one of two side slots of the CTA, and the
-// joining kernel adds the parts up in order; there are no atomics.
+// lengths (4 bytes a sequence) and finds its warps' first units.  Where a warp's
+// range cuts a sequence, its part goes to one of two side slots of the warp, and
+// the joining kernel adds the parts up in order; there are no atomics, and no
+// warp waits for another one (with a CTA per range, its four warps joined at the
+// end of every sequence, 2048 short segments took 77 us instead of XXX).
 //
-// Four warps, 32 keys each per unit, each with a ring of its own that TMA fills
-// from the pages DC_DEPTH units ahead, across the ends of sequences.  Per 32
-// keys, on mma.sync m16n8k16 with the keys (and the head dimensions) on the 16
-// rows, the 8 columns being query heads:
+// Each warp has a ring of its own, K and V of a unit in turn, that TMA fills from
+// the pages, across the ends of sequences.  Per unit, on mma.sync m16n8k16 with the
+// keys (and the head dimensions) on the 16 rows, the 8 columns being query heads:
 //   S^T[key, head]  = K q^T            ldmatrix of K as it lies
 //   O^T[dim, head] += V^T P^T          ldmatrix.trans of V as it lies; P^T from
 //                                      the accumulator layout by movmatrix
@@ -29,28 +30,28 @@
 
 namespace ddq {
 
-constexpr int DC_NW = 4;
-constexpr int DC_UNIT = 32 * DC_NW;  // keys
-constexpr int DC_DEPTH = 3;
-constexpr int DC_SCAN = 64;          // sequences a thread sums at most
+constexpr int DC_NW = 8;             // warps: two a quarter of the SM hide each other's latency
+constexpr int DC_UNIT = 32;          // keys
+constexpr int DC_SLOTS = 3;          // of 32 rows of K or of V in turn, per warp
+constexpr int DC_SCAN = 32;          // sequences a thread sums at most
 constexpr int DC_MAXB = DC_SCAN * DC_NW * 32;
 
-// Side slots (2 per CTA), and for each segment (sequence, key/value head, head
-// group) the CTAs that hold its first and its last unit.
+// Side slots (2 per warp), and for each segment (sequence, key/value head, head
+// group) the warps that hold its first and its last unit.
 struct DcSide {
-  float* o;      // [2 N][heads][D]
-  float* lse;    // [2 N][heads]
+  float* o;      // [2 N][16][D]
+  float* lse;    // [2 N][16]
   int2* seg;     // [B * Hkv * groups]
 };
 
-template <int D, int NB>
+template <int D>
 struct DcSmem {
-  uint8_t ring[DC_NW * DC_DEPTH][2][32 * D * 2];
-  float acc[DC_NW][8 * NB][D];
-  float m[DC_NW][8 * NB], l[DC_NW][8 * NB];
-  unsigned long long full[DC_NW * DC_DEPTH];
+  uint8_t ring[DC_NW * DC_SLOTS][32 * D * 2];
+  float out[DC_NW][8][D + 4];  // a warp's results of 8 heads on their way out
+  unsigned long long full[DC_NW * DC_SLOTS];
   long long wsum[DC_NW];
-  int start[4];
+  int most[DC_NW];
+  int start[DC_NW][4];
   int abort_flag;
 };
 
@@ -102,21 +103,30 @@ __device__ __forceinline__ void dc_mma<__nv_bfloat16>(float* d, const uint32_t* 
 // byte offset of 16-byte piece j of row r in a tile of 64 elements a row
 __device__ __forceinline__ uint32_t dc_swz(int r, int j) { return r * 128 + ((j ^ (r & 7)) << 4); }
 
+// CTAs of an SM: shared memory (113 KB, 228 KB) and registers
+__host__ __device__ constexpr int dc_resident(int d, int nb) { return d == 64 && nb == 1 ? 2 : 1; }
+
 __host__ __device__ __forceinline__ int dc_groups(int G) { return (G + 15) / 16; }
 
 // A position in the list of units.
 struct DcWalk {
-  int b, seg, c;   // sequence, key/value head and head group, unit of the sequence
-  int len, units;  // of the sequence
+  int b, g, grp, c;  // sequence, key/value head, head group, unit of the sequence
+  int len, units;    // of the sequence
 };
 
+// x / d where x mostly fits 32 bits (a 64-bit division takes some 150 instructions)
+__device__ __forceinline__ long long dc_div(long long x, long long d) {
+  if (((x | d) >> 32) == 0) return (uint32_t)x / (uint32_t)d;
+  return x / d;
+}
+
 template <typename E, int D, int NB>
-__global__ void __launch_bounds__(DC_NW * 32)
+__global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
     paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const PgAttnArgs a,
                         const PgParts parts, const DcSide side, const unsigned long long tmo) {
   using Ty = PgType<E>;
-  using Sm = DcSmem<D, NB>;
+  using Sm = DcSmem<D>;
   constexpr int H2 = D / 64;
   constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ uint8_t dc_raw[];
@@ -127,9 +137,8 @@ __global__ void __launch_bounds__(DC_NW * 32)
   const int G = a.Hq / a.c.Hkv, groups = dc_groups(G), segs = a.c.Hkv * groups;
   const bool prefix = a.prefix_len > 0;
   if (tid == 0) {
-    for (int s = 0; s < DC_NW * DC_DEPTH; ++s) ptx::mbar_init(ptx::smem_u32(&sm.full[s]), 1);
+    for (int s = 0; s < DC_NW * DC_SLOTS; ++s) ptx::mbar_init(ptx::smem_u32(&sm.full[s]), 1);
     sm.abort_flag = 0;
-    sm.start[0] = -1;
     ptx::fence_mbar_init();
     ptx::prefetch_tmap(&tm_k);
     ptx::prefetch_tmap(&tm_v);
@@ -141,47 +150,70 @@ __global__ void __launch_bounds__(DC_NW * 32)
   if (!prefix) ptx::pdl_wait();
   ptx::pdl_launch_dependents();
 
-  // ---- this CTA's units
+  // ---- this warp's units
   auto units_of = [&](int len) { return max(1, (len + DC_UNIT - 1) / DC_UNIT); };
   const int per = (a.R + DC_NW * 32 - 1) / (DC_NW * 32);  // sequences a thread sums
   const int b0 = min(tid * per, a.R), b1 = min(b0 + per, a.R);
   long long sum = 0;
-  for (int b = b0; b < b1; ++b) sum += units_of(pg_len(a, b));
+  int most = 0;  // units of the longest sequence
+  for (int b = b0; b < b1; ++b) {
+    const int n = units_of(pg_len(a, b));
+    sum += n;
+    most = max(most, n);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
   long long inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long u = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += u;
   }
-  if (lane == 31) sm.wsum[warp] = inc;
+  if (lane == 31) {
+    sm.wsum[warp] = inc;
+    sm.most[warp] = most;
+  }
   __syncthreads();
   long long total = 0;
 #pragma unroll
   for (int w = 0; w < DC_NW; ++w) {
     if (w < warp) inc += sm.wsum[w];
     total += sm.wsum[w];
+    most = max(most, sm.most[w]);
   }
   total *= segs;
-  // (with fewer units than CTAs the first `total` take one each: the parts of a
-  // sequence lie in consecutive CTAs, none of them empty)
-  const long long N = min((long long)gridDim.x, total);
-  const long long u0 = total * blockIdx.x / N, u1 = total * (blockIdx.x + 1) / N;
-  if (blockIdx.x >= N) {
+  // With few units the first warps take `least` each (the parts of a sequence lie
+  // in consecutive warps, none of them empty): a unit more costs a warp 0.35 us, 32
+  // parts more cost the joining 0.8 us, so least^2 = most / 14 or so.
+  const int least = max(1, (int)(sqrtf((float)most * 0.0625f) + 0.5f));
+  const long long N = max(1ll, min((long long)gridDim.x * DC_NW, total / least));
+  const long long w0 = (long long)blockIdx.x * DC_NW;
+  if (w0 >= N) {
     if (prefix) ptx::pdl_wait();
     return;
   }
-  long long at = (inc - sum) * segs;
-  if (u0 >= at && u0 < inc * segs) {
+  // warp i starts at unit i q + min(i, r): the first r take one more
+  const long long uq = dc_div(total, N), ur = total - uq * N;
+  for (int w = 0; w < DC_NW && w0 + w < N; ++w) {
+    const long long u0 = (w0 + w) * uq + min(w0 + w, ur);
+    long long at = (inc - sum) * segs;
+    if (u0 < at || u0 >= inc * segs) continue;
     int b = b0, n = units_of(pg_len(a, b));
     while (u0 >= at + (long long)n * segs) {
       at += (long long)n * segs;
       n = units_of(pg_len(a, ++b));
     }
-    sm.start[0] = b;
-    sm.start[1] = (int)((u0 - at) / n);
-    sm.start[2] = (int)((u0 - at) % n);
+    const int seg = (int)dc_div(u0 - at, n);
+    sm.start[w][0] = b;
+    sm.start[w][1] = seg / groups;
+    sm.start[w][2] = seg % groups;
+    sm.start[w][3] = (int)(u0 - at - (long long)seg * n);
   }
   __syncthreads();
+  if (w0 + warp >= N) {
+    if (prefix) ptx::pdl_wait();
+    return;
+  }
+  const int worker = (int)w0 + warp;
   auto load_len = [&](DcWalk& w) {
     w.len = w.b < a.R ? pg_len(a, w.b) : 0;
     w.units = units_of(w.len);
@@ -189,36 +221,40 @@ __global__ void __launch_bounds__(DC_NW * 32)
   auto advance = [&](DcWalk& w) {
     if (++w.c < w.units) return;
     w.c = 0;
-    if (++w.seg < segs) return;
-    w.seg = 0;
+    if (++w.grp < groups) return;
+    w.grp = 0;
+    if (++w.g < a.c.Hkv) return;
+    w.g = 0;
     ++w.b;
     load_len(w);
   };
-  DcWalk cw{sm.start[0], sm.start[1], sm.start[2], 0, 0};
+  DcWalk cw{sm.start[warp][0], sm.start[warp][1], sm.start[warp][2], sm.start[warp][3], 0, 0};
   load_len(cw);
-  const int count = (int)(u1 - u0);
+  const int count = (int)(uq + (worker < ur ? 1 : 0));
 
   // ---- loads: chunk after chunk of this warp, the page numbers one ahead
   const int br = min(1 << a.c.page_shift, 32), nb = 32 / br;  // rows of a box, boxes of 32 keys
-  const int sub = lane % nb, dh = (lane / nb) % H2, kv = lane / (nb * H2);
-  const uint32_t ring = ptx::smem_u32(&sm.ring[warp * DC_DEPTH][0][0]);
-  const uint32_t bar = ptx::smem_u32(&sm.full[warp * DC_DEPTH]);
+  const int sub = lane % nb, dh = lane / nb;
+  const uint32_t ring = ptx::smem_u32(&sm.ring[warp * DC_SLOTS][0]);
+  const uint32_t bar = ptx::smem_u32(&sm.full[warp * DC_SLOTS]);
+  constexpr uint32_t SLOT = 32 * D * 2;
   DcWalk lw = cw;
-  int ahead = 0;        // units that lw is past u0
-  int issued = 0;       // chunks requested
+  int ahead = 0;        // units that lw is past the first
+  int is = 0;           // the slot to fill next
+  int issued = 0;
+  bool pend_v = false;  // the unit's K has been requested, its V is next
   int pend_page = 0, pend_row = 0, pend_head = 0;
   bool pend_mine = false, pend = false;
-  auto look = [&] {     // the next chunk with keys: its page number, not used yet
+  auto look = [&] {     // the next unit with keys: its page number, not used yet
     pend = false;
     while (ahead < count) {
-      const int base = lw.c * DC_UNIT + warp * 32;
+      const int base = lw.c * DC_UNIT;
       if (base < lw.len) {
         const int key = base + sub * br;
-        pend_mine = kv < 2 && key < lw.len;
-        if (pend_mine)
-          pend_page = a.table[lw.b * a.table_stride + (key >> a.c.page_shift)];
+        pend_mine = dh < H2 && key < lw.len;
+        if (pend_mine) pend_page = a.table[lw.b * a.table_stride + (key >> a.c.page_shift)];
         pend_row = key & ((1 << a.c.page_shift) - 1);
-        pend_head = lw.seg / groups;
+        pend_head = lw.g;
         pend = true;
         advance(lw);
         ++ahead;
@@ -228,23 +264,22 @@ __global__ void __launch_bounds__(DC_NW * 32)
       ++ahead;
     }
   };
-  auto issue = [&] {    // the chunk looked up into the next slot
-    const int s = issued % DC_DEPTH;
-    bool mine = pend_mine;
-    if (mine) mine = pg_check(a.c, pend_page) >= 0;
-    const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, mine)) * br * 128u;
-    if (lane == 0) ptx::mbar_arrive_expect_tx(bar + 8 * s, bytes);
+  auto issue = [&] {    // K or V of the unit looked up into the next slot
+    if (!pend_v && pend_mine) pend_mine = pg_check(a.c, pend_page) >= 0;
+    const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, pend_mine)) * br * 128u;
+    if (lane == 0) ptx::mbar_arrive_expect_tx(bar + 8 * is, bytes);
     __syncwarp();
-    if (mine)
-      ptx::tma_load_4d(ring + (uint32_t)(((s * 2 + kv) * H2 + dh) * 4096 + sub * br * 128),
-                       kv ? &tm_v : &tm_k, dh * 64, pend_row, pend_head, pend_page, bar + 8 * s);
+    if (pend_mine)
+      ptx::tma_load_4d(ring + is * SLOT + (uint32_t)(dh * 4096 + sub * br * 128),
+                       pend_v ? &tm_v : &tm_k, dh * 64, pend_row, pend_head, pend_page,
+                       bar + 8 * is);
+    is = is + 1 == DC_SLOTS ? 0 : is + 1;
     ++issued;
+    if (pend_v) look();
+    pend_v = !pend_v;
   };
   look();
-  for (int i = 0; i < DC_DEPTH && pend; ++i) {
-    issue();
-    look();
-  }
+  for (int i = 0; i < DC_SLOTS && pend; ++i) issue();
 
   // ---- compute
   const bool plain = a.cap == 0.f && a.slopes == nullptr && a.scale > 0.f;
@@ -253,9 +288,9 @@ __global__ void __launch_bounds__(DC_NW * 32)
   float m[NB][2], l[NB][2], slope[NB][2], o[D / 16][NB][4];
   // the queries of a segment, requested while the segment before it is joined
   auto load_q = [&](const DcWalk& w) {
-    const int grp = w.seg % groups, heads = min(16, G - grp * 16);
+    const int heads = min(16, G - w.grp * 16);
     const E* base = reinterpret_cast<const E*>(a.q) + w.b * a.q_ts + col2;
-    const int first = w.seg / groups * G + grp * 16;
+    const int first = w.g * G + w.grp * 16;
 #pragma unroll
     for (int nbk = 0; nbk < NB; ++nbk) {
       const int hq = row4 + 8 * nbk;
@@ -269,12 +304,35 @@ __global__ void __launch_bounds__(DC_NW * 32)
   };
   load_q(cw);
   bool fresh = true;      // the next unit starts a part of a segment
-  bool whole = true;      // ... which begins in this CTA
+  bool whole = true;      // ... which begins in this warp
+  int us = 0;             // the slot in use, and its phase
+  uint32_t phase = 0;
   int used = 0;
   bool dead = false;
+  // the slot's copy has landed / the slot is free: the next copy into it
+  auto take = [&] {
+    dead = !__all_sync(0xffffffffu, ptx::mbar_wait(bar + 8 * us, phase, tmo, &sm.abort_flag));
+  };
+  auto give = [&] {
+    __syncwarp();
+    ++used;
+    us = us + 1 == DC_SLOTS ? 0 : us + 1;
+    if (us == 0) phase ^= 1u;
+    if (pend) {
+      ptx::fence_proxy_async_smem();
+      issue();
+    }
+  };
+  // shared-memory offsets of this lane's matrix rows: 16 of K, 8 + 8 of V
+  uint32_t ko[4], vo[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    ko[e] = dc_swz(lane & 15, 2 * e + (lane >> 4));
+    vo[e] = dc_swz((lane & 7) + 8 * (lane >> 4), 2 * e + ((lane >> 3) & 1));
+  }
   for (int u = 0; u < count; ++u) {
-    const int g = cw.seg / groups, h0 = g * G + (cw.seg % groups) * 16;  // first query head
-    const int heads = min(16, G - (cw.seg % groups) * 16);
+    const int h0 = cw.g * G + cw.grp * 16;  // first query head
+    const int heads = min(16, G - cw.grp * 16);
     if (fresh) {
       fresh = false;
       whole = cw.c == 0;
@@ -292,22 +350,12 @@ __global__ void __launch_bounds__(DC_NW * 32)
           o[e][nbk][0] = o[e][nbk][1] = o[e][nbk][2] = o[e][nbk][3] = 0.f;
       }
     }
-    const int base = cw.c * DC_UNIT + warp * 32;
+    const int base = cw.c * DC_UNIT;
     const int have = min(32, cw.len - base);
     if (have > 0 && !dead) {
-      const int s = used % DC_DEPTH;
-      dead = !__all_sync(0xffffffffu, ptx::mbar_wait(bar + 8 * s, (uint32_t)(used / DC_DEPTH) & 1u,
-                                                     tmo, &sm.abort_flag));
+      take();
       if (!dead) {
-        const uint32_t ks = ring + (uint32_t)(s * 2 * H2 * 4096), vs = ks + H2 * 4096;
-        if (have < 32) {  // rows behind the last key may hold anything: 0 x NaN is NaN
-          uint8_t* vr = &sm.ring[warp * DC_DEPTH + s][1][0];
-          for (int x = have * 8 + lane; x < 32 * 8; x += 32)
-#pragma unroll
-            for (int hb = 0; hb < H2; ++hb)
-              *reinterpret_cast<uint4*>(vr + hb * 4096 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-          __syncwarp();
-        }
+        const uint32_t ks = ring + us * SLOT;
         // S^T: keys 16 mt + row4 (+ 8), heads col2 (+ 1)
         float sc[2][NB][4];
 #pragma unroll
@@ -318,13 +366,13 @@ __global__ void __launch_bounds__(DC_NW * 32)
 #pragma unroll
           for (int e = 0; e < D / 16; ++e) {
             uint32_t r[4];
-            dc_ldsm(ks + (e >> 2) * 4096 +
-                        dc_swz(16 * mt + (lane & 15), 2 * (e & 3) + (lane >> 4)), r);
+            dc_ldsm(ks + (e >> 2) * 4096 + mt * 2048 + ko[e & 3], r);
 #pragma unroll
             for (int nbk = 0; nbk < NB; ++nbk)
               dc_mma<E>(sc[mt][nbk], r, q[nbk][e][0], q[nbk][e][1]);
           }
         }
+        give();
         bool grow = false;
         float mx[NB][2];
 #pragma unroll
@@ -390,25 +438,29 @@ __global__ void __launch_bounds__(DC_NW * 32)
             pb[mt][nbk][0] = dc_transpose(Ty::pack(p0, p1));
             pb[mt][nbk][1] = dc_transpose(Ty::pack(p2, p3));
           }
-        // O^T: dims 16 e + row4 (+ 8), heads col2 (+ 1)
+        take();
+        if (!dead) {
+          const uint32_t vs = ring + us * SLOT;
+          if (have < 32) {  // rows behind the last key may hold anything: 0 x NaN is NaN
+            uint8_t* vr = &sm.ring[warp * DC_SLOTS + us][0];
+            for (int x = have * 8 + lane; x < 32 * 8; x += 32)
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e)
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
-            uint32_t r[4];
-            dc_ldsm_t(vs + (e >> 2) * 4096 + dc_swz(16 * mt + (lane & 7) + 8 * (lane >> 4),
-                                                    2 * (e & 3) + ((lane >> 3) & 1)), r);
-#pragma unroll
-            for (int nbk = 0; nbk < NB; ++nbk)
-              dc_mma<E>(o[e][nbk], r, pb[mt][nbk][0], pb[mt][nbk][1]);
+              for (int hb = 0; hb < H2; ++hb)
+                *reinterpret_cast<uint4*>(vr + hb * 4096 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+            __syncwarp();
           }
-        ++used;
-        // the slot is free: the next chunk into it
-        __syncwarp();
-        if (pend) {
-          ptx::fence_proxy_async_smem();
-          issue();
-          look();
+          // O^T: dims 16 e + row4 (+ 8), heads col2 (+ 1)
+#pragma unroll
+          for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+              uint32_t r[4];
+              dc_ldsm_t(vs + (e >> 2) * 4096 + mt * 2048 + vo[e & 3], r);
+#pragma unroll
+              for (int nbk = 0; nbk < NB; ++nbk)
+                dc_mma<E>(o[e][nbk], r, pb[mt][nbk][0], pb[mt][nbk][1]);
+            }
+          give();
         }
       }
     }
@@ -416,73 +468,65 @@ __global__ void __launch_bounds__(DC_NW * 32)
     const DcWalk now = cw;
     advance(cw);
     if (cw.c != 0 && u + 1 < count) continue;
-    // ---- the end of this CTA's part of the segment: the warps' results, joined
+    // ---- the end of this warp's part of the segment
     fresh = true;
     if (u + 1 < count) load_q(cw);
+    const bool done = now.c == now.units - 1;     // the part has the segment's last unit
+    const bool full = whole && done;
+    if (lane == 0) {
+      int2* info = side.seg + (int64_t)now.b * segs + now.g * groups + now.grp;
+      if (whole) info->x = worker;
+      if (done) info->y = worker;
+    }
+    const int slot = 2 * worker + (whole ? 1 : 0);
+    // where head h of the group goes, if not to the output: row of parts or side
+    auto part_row = [&](int h) {
+      return full ? (int64_t)(parts.count - 1) * parts.rows + (int64_t)now.b * a.Hq + h0 + h
+                  : (int64_t)slot * 16 + h;
+    };
+    float* const po = full ? parts.o : side.o;
+    float* const pl = full ? parts.lse : side.lse;
+    const bool direct = full && !prefix;
 #pragma unroll
-    for (int nbk = 0; nbk < NB; ++nbk)
+    for (int nbk = 0; nbk < NB; ++nbk) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         float v = l[nbk][x];
 #pragma unroll
         for (int sh = 4; sh < 32; sh <<= 1) v += __shfl_xor_sync(0xffffffffu, v, sh);
-        if (row4 == 0) {
-          sm.m[warp][8 * nbk + col2 + x] = m[nbk][x];
-          sm.l[warp][8 * nbk + col2 + x] = v;
-        }
+        const float inv = v == 0.f ? 0.f : 1.f / v;  // no keys: 0; a NaN goes on
+        const int h = 8 * nbk + col2 + x;
+        if (row4 == 0 && h < heads && !direct)
+          pl[part_row(h)] = v == 0.f ? -INFINITY : m[nbk][x] + log2f(v);
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) {
-          sm.acc[warp][8 * nbk + col2 + x][16 * e + row4] = o[e][nbk][x];
-          sm.acc[warp][8 * nbk + col2 + x][16 * e + row4 + 8] = o[e][nbk][2 + x];
+          sm.out[warp][col2 + x][16 * e + row4] = o[e][nbk][x] * inv;
+          sm.out[warp][col2 + x][16 * e + row4 + 8] = o[e][nbk][2 + x] * inv;
         }
       }
-    __syncthreads();
-    const bool done = now.c == now.units - 1;     // the part has the segment's last unit
-    const bool full = whole && done;
-    if (tid == 0) {
-      int2* info = side.seg + (int64_t)now.b * segs + now.seg;
-      if (whole) info->x = blockIdx.x;
-      if (done) info->y = blockIdx.x;
-    }
-    const int slot = 2 * blockIdx.x + (whole ? 1 : 0);
-    for (int i = tid; i < heads * (D / 2); i += DC_NW * 32) {
-      const int h = i / (D / 2), d = 2 * (i % (D / 2));
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < DC_NW; ++w) top = fmaxf(top, sm.m[w][h]);
-      float den = 0.f, v0 = 0.f, v1 = 0.f;
-#pragma unroll
-      for (int w = 0; w < DC_NW; ++w) {
-        const float lw_ = sm.l[w][h];
-        if (lw_ == 0.f) continue;  // no keys (a NaN goes on)
-        const float c = dc_exp2(sm.m[w][h] == top ? 0.f : sm.m[w][h] - top);
-        const float2 av = *reinterpret_cast<const float2*>(&sm.acc[w][h][d]);
-        den = fmaf(lw_, c, den);
-        v0 = fmaf(av.x, c, v0);
-        v1 = fmaf(av.y, c, v1);
+      __syncwarp();
+      for (int i = lane; i < min(8, heads - 8 * nbk) * (D / 8); i += 32) {
+        const int hr = i / (D / 8), h = 8 * nbk + hr, d = 8 * (i % (D / 8));
+        const float4 v = *reinterpret_cast<const float4*>(&sm.out[warp][hr][d]);
+        const float4 w = *reinterpret_cast<const float4*>(&sm.out[warp][hr][d + 4]);
+        if (direct) {
+          *reinterpret_cast<uint4*>(reinterpret_cast<E*>(a.out) + now.b * a.o_ts +
+                                    (int64_t)(h0 + h) * a.o_hs + d) =
+              make_uint4(Ty::pack(v.x, v.y), Ty::pack(v.z, v.w), Ty::pack(w.x, w.y),
+                         Ty::pack(w.z, w.w));
+        } else {
+          float* dst = po + part_row(h) * D + d;
+          *reinterpret_cast<float4*>(dst) = v;
+          *reinterpret_cast<float4*>(dst + 4) = w;
+        }
       }
-      const float inv = den == 0.f ? 0.f : 1.f / den;
-      const float lse = den == 0.f ? -INFINITY : top + log2f(den);
-      const int64_t row = (int64_t)now.b * a.Hq + h0 + h;
-      if (full && !prefix) {
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<E*>(a.out) + now.b * a.o_ts +
-                                     (int64_t)(h0 + h) * a.o_hs + d) = Ty::pack(v0 * inv, v1 * inv);
-      } else if (full) {
-        const int64_t pr = (int64_t)(parts.count - 1) * parts.rows + row;
-        *reinterpret_cast<float2*>(parts.o + pr * D + d) = make_float2(v0 * inv, v1 * inv);
-        if (d == 0) parts.lse[pr] = lse;
-      } else {
-        const int64_t pr = (int64_t)slot * 16 + h;
-        *reinterpret_cast<float2*>(side.o + pr * D + d) = make_float2(v0 * inv, v1 * inv);
-        if (d == 0) side.lse[pr] = lse;
-      }
+      __syncwarp();  // sm.out is free again
     }
-    __syncthreads();  // acc, m and l are free again
   }
   if (dead) {         // copies in flight land before the shared memory goes
     for (int k = used; k < issued; ++k) {
       const long long t0 = clock64();
-      while (!ptx::mbar_try_wait(bar + 8 * (k % DC_DEPTH), (uint32_t)(k / DC_DEPTH) & 1u))
+      while (!ptx::mbar_try_wait(bar + 8 * (k % DC_SLOTS), (uint32_t)(k / DC_SLOTS) & 1u))
         if (clock64() - t0 > (long long)(tmo * 2ull)) break;
     }
     if (lane == 0) pg_error(a.c, DDQ_ERR_TIMEOUT);
@@ -491,10 +535,10 @@ __global__ void __launch_bounds__(DC_NW * 32)
 }
 
 // Joins the parts of every row, in order: the prefix splits, then the own keys
-// (whole, or the side slots of the CTAs that share them).
+// (whole, or the side slots of the warps that share them).
 //   o = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z - max)
-// One warp per row.
-template <typename E, int D>
+// One warp per row, or, with few rows (of long sequences: many parts), eight.
+template <typename E, int D, int WPR>
 __global__ void __launch_bounds__(256)
     paged_decode_merge_kernel(const PgAttnArgs a, const PgParts p, const DcSide side) {
   using Ty = PgType<E>;
@@ -502,7 +546,8 @@ __global__ void __launch_bounds__(256)
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int warp = threadIdx.x >> 5;
+  const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;
   if (row >= (int64_t)a.T * a.Hq) return;
   const int b = (int)(row / a.Hq), h = (int)(row % a.Hq);
   const int G = a.Hq / a.c.Hkv, groups = dc_groups(G);
@@ -530,7 +575,7 @@ __global__ void __launch_bounds__(256)
     const float ls = lse_of(z0 + lane);
     const float wl = ls == -INFINITY ? 0.f : exp2f(ls - mx);
     const int m = min(32, n - z0);
-    for (int z1 = 0; z1 < m; z1 += 4) {  // four parts in flight
+    for (int z1 = WPR == 1 ? 0 : 4 * warp; z1 < m; z1 += 4 * WPR) {  // four in flight
       float v[4][DPL], w[4];
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
@@ -556,6 +601,20 @@ __global__ void __launch_bounds__(256)
       }
     }
   }
+  if constexpr (WPR > 1) {
+    __shared__ float so[WPR][D], sd[WPR];
+#pragma unroll
+    for (int e = 0; e < DPL; ++e) so[warp][lane * DPL + e] = o[e];
+    if (lane == 0) sd[warp] = den;
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) {
+      den += sd[w];
+#pragma unroll
+      for (int e = 0; e < DPL; ++e) o[e] += so[w][lane * DPL + e];
+    }
+  }
   const float inv = den == 0.f ? 0.f : 1.f / den;  // NaN stays NaN
   E* dst = reinterpret_cast<E*>(a.out) + b * a.o_ts + (int64_t)h * a.o_hs + lane * DPL;
 #pragma unroll
@@ -563,13 +622,14 @@ __global__ void __launch_bounds__(256)
     *reinterpret_cast<uint32_t*>(dst + e) = Ty::pack(o[e] * inv, o[e + 1] * inv);
 }
 
-template <int D, int NB>
-constexpr int dc_smem_bytes() { return (int)sizeof(DcSmem<D, NB>) + 1024; }
+template <int D>
+constexpr int dc_smem_bytes() { return (int)sizeof(DcSmem<D>) + 1024; }
 
-// CTAs that fit the GPU at once: two per SM with 64-wide heads (105 KB each).
+// CTAs that fit the GPU at once.
 int dc_ctas(int64_t B, int Hq, int Hkv, int D, int64_t keys, int sms) {
-  const int64_t most = B * Hkv * dc_groups(Hq / Hkv) * ((keys + DC_UNIT - 1) / DC_UNIT);
-  const int64_t fit = (int64_t)sms * (D == 64 ? 2 : 1);
+  const int64_t units = B * Hkv * dc_groups(Hq / Hkv) * ((keys + DC_UNIT - 1) / DC_UNIT);
+  const int64_t most = (units + DC_NW - 1) / DC_NW;
+  const int64_t fit = (int64_t)sms * dc_resident(D, Hq / Hkv > 8 ? 2 : 1);
   return (int)(most < 1 ? 1 : most < fit ? most : fit);
 }
 
@@ -580,8 +640,8 @@ DcPlan dc_plan(int64_t B, int Hq, int Hkv, int D, int64_t keys, int64_t prefix, 
   const int64_t rows = B * Hq, count = prefix ? p.splits + 1 : 0;
   p.off_lse = (size_t)count * rows * D * 4;
   p.off_so = p.off_lse + ((size_t)count * rows * 4 + 15) / 16 * 16;
-  p.off_sl = p.off_so + (size_t)p.ctas * 2 * 16 * D * 4;
-  p.off_seg = p.off_sl + (size_t)p.ctas * 2 * 16 * 4;
+  p.off_sl = p.off_so + (size_t)p.ctas * DC_NW * 2 * 16 * D * 4;
+  p.off_seg = p.off_sl + (size_t)p.ctas * DC_NW * 2 * 16 * 4;
   p.bytes = p.off_seg + (size_t)B * Hkv * dc_groups(Hq / Hkv) * sizeof(int2);
   return p;
 }
@@ -629,9 +689,9 @@ int launch_paged_decode(const PgAttnArgs& a, bool bf16, void* ws, const DcPlan& 
   const bool wide = a.Hq / a.c.Hkv > 8;
 #define DDQ_DC(D_, NB_)                                                                        \
   (bf16 ? go(paged_decode_kernel<__nv_bfloat16, D_, NB_>, attr[1][D_ / 128][NB_ - 1],          \
-             dc_smem_bytes<D_, NB_>())                                                         \
+             dc_smem_bytes<D_>())                                                         \
         : go(paged_decode_kernel<__half, D_, NB_>, attr[0][D_ / 128][NB_ - 1],                 \
-             dc_smem_bytes<D_, NB_>()))
+             dc_smem_bytes<D_>()))
   if (a.c.D == 64)
     st = wide ? DDQ_DC(64, 2) : DDQ_DC(64, 1);
   else
@@ -639,17 +699,19 @@ int launch_paged_decode(const PgAttnArgs& a, bool bf16, void* ws, const DcPlan& 
 #undef DDQ_DC
   if (st) return st;
   if (e == cudaSuccess) {
-    cfg.gridDim = dim3((unsigned)(((int64_t)a.T * a.Hq + 7) / 8));
+    const int64_t rows = (int64_t)a.T * a.Hq;
+    const bool few = rows <= 16 * (int64_t)device_sm_count(dev);
+    cfg.gridDim = dim3((unsigned)(few ? rows : (rows + 7) / 8));
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
+#define DDQ_DM(E_, D_)                                                                        \
+  (few ? cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<E_, D_, 8>, a, parts, side)       \
+       : cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<E_, D_, 1>, a, parts, side))
     if (bf16)
-      e = a.c.D == 64
-              ? cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<__nv_bfloat16, 64>, a, parts, side)
-              : cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<__nv_bfloat16, 128>, a, parts, side);
+      e = a.c.D == 64 ? DDQ_DM(__nv_bfloat16, 64) : DDQ_DM(__nv_bfloat16, 128);
     else
-      e = a.c.D == 64
-              ? cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<__half, 64>, a, parts, side)
-              : cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<__half, 128>, a, parts, side);
+      e = a.c.D == 64 ? DDQ_DM(__half, 64) : DDQ_DM(__half, 128);
+#undef DDQ_DM
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
