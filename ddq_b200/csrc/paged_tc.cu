@@ -81,6 +81,21 @@ __device__ __forceinline__ float tc_rcp(float x) {
   return y;
 }
 
+__device__ __forceinline__ void tc_sts(uint32_t p, uint32_t a, uint32_t b, uint32_t c,
+                                       uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+
+__device__ __forceinline__ uint4 tc_lds(uint32_t p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(p)
+               : "memory");
+  return v;
+}
+
 __device__ __forceinline__ void tc_regs(uint32_t* r) {  // the loads above are complete
 #pragma unroll
   for (int i = 0; i < 32; i += 8)
@@ -144,14 +159,12 @@ __device__ __forceinline__ TcF2 tc_poly_exp2(float x0, float x1) {
 // buffers hold, and no lane leaves its warp in between.  A wait on a phase that
 // is complete costs 55 cycles this way; with an answer for the warp to branch on
 // it cost 106, six times per pair of tiles on the path from P to the next S.
-// (Short on purpose: the warps of a quarter of the SM share a small instruction
-// cache.  The limit is in polls of at least 50 cycles, so a wait at lower clocks
-// only lasts longer.)
-__device__ __forceinline__ void tc_wait(uint32_t bar, uint32_t parity, uint32_t polls,
+__device__ __forceinline__ void tc_wait(uint32_t bar, uint32_t parity, uint64_t tmo,
                                         volatile int* abort) {
   if (!ptx::mbar_try_wait_now(bar, parity)) {
+    const long long t0 = clock64();
     while (!ptx::mbar_try_wait(bar, parity)) {
-      if (*abort || --polls == 0) {
+      if (*abort || clock64() - t0 > (long long)(tmo * 2ull)) {
         *abort = 1;
         break;
       }
@@ -185,7 +198,6 @@ __global__ void __launch_bounds__(TC_NT, 1)
                                              ~static_cast<uintptr_t>(1023));
   const uint32_t sbase = ptx::smem_u32(smem);
   __shared__ int found[6], wsum[TC_NT / 32];  // request, tile, first row, rows, keys, bidir
-  const uint32_t polls = (uint32_t)min(tmo / 25ull + 1ull, 0xffffffffull);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.Hq / a.c.Hkv, g = blockIdx.y, z = blockIdx.z;
 
@@ -221,9 +233,15 @@ __global__ void __launch_bounds__(TC_NT, 1)
     ptx::prefetch_tmap(&tm_k);
     ptx::prefetch_tmap(&tm_v);
   }
+  if (warp == 9) {
+    ptx::tmem_alloc(ptx::smem_u32(tmem_holder), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
-  __syncthreads();
 
   // ---- the request and the tile of this CTA: requests and their tiles from the
   // last to the first, so that the CTAs that start last have the fewest keys
@@ -269,7 +287,10 @@ __global__ void __launch_bounds__(TC_NT, 1)
       if (found[0] >= 0) break;
     }
     r = found[0];
-    if (r < 0) return;  // the grid covers the most tiles that T rows can make
+    if (r < 0) {  // the grid covers the most tiles that T rows can make
+      if (warp == 9) ptx::tmem_dealloc(*tmem_holder, 512);
+      return;
+    }
     tile = found[1];
     t_first = found[2];
     n = found[3];
@@ -304,16 +325,10 @@ __global__ void __launch_bounds__(TC_NT, 1)
           *reinterpret_cast<uint4*>(dst + c) = make_uint4(0u, 0u, 0u, 0u);
       }
     }
+    if (warp == 9) ptx::tmem_dealloc(*tmem_holder, 512);
     return;
   }
 
-  if (warp == 9) {
-    ptx::tmem_alloc(ptx::smem_u32(tmem_holder), 512);
-    ptx::tmem_relinquish();
-  }
-  ptx::tc_fence_before();
-  __syncthreads();
-  ptx::tc_fence_after();
   const uint32_t tmem = *tmem_holder;
 
   if (warp < 8) {
@@ -372,7 +387,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
         const int j0 = key0(k);
         const int lim = min(end, limit(k)) - j0;  // keys of this tile that the row attends
         const bool full = __all_sync(0xffffffffu, lim >= TC_KV);
-        tc_wait(bar_s + 8 * t, (uint32_t)k & 1u, polls, abort_flag);
+        tc_wait(bar_s + 8 * t, (uint32_t)k & 1u, tmo, abort_flag);
         ptx::tc_fence_after();
         // the row into registers, and S is free for the next scores
         uint32_t u[128];
@@ -459,7 +474,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
             l *= alpha;
           }
           if (k > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, polls, abort_flag);
+            tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
             ptx::tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
@@ -502,7 +517,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
         for (int hf = 0; hf < 2; ++hf) {
           if (full && plain) weights(hf, std::true_type()); else weights(hf, std::false_type());
           if (hf == 0 && k > 0) {  // P of the tile before has been read
-            tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, polls, abort_flag);
+            tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
             ptx::tc_fence_after();
           }
           ptx::tmem_st_32x32b_x32(tp + 32 * hf, u + 32 * hf);
@@ -516,11 +531,13 @@ __global__ void __launch_bounds__(TC_NT, 1)
           l += l0 + l1;
         }
       }
-      tc_wait(bar_pv + 8 * t, (uint32_t)(cnt - 1) & 1u, polls, abort_flag);
+      tc_wait(bar_pv + 8 * t, (uint32_t)(cnt - 1) & 1u, tmo, abort_flag);
       ptx::tc_fence_after();
     }
-    // ---- O / l, or the split's part of it.  Every lane takes part in the TMEM
-    // loads; a half without rows, and a row behind the last, stores nothing.
+    // ---- O / l, or the split's part of it, through the shared memory of the warp's
+    // rows of Q (all scores are made): 8 lanes store 128 bytes of a row together.
+    // Every lane takes part in the TMEM loads; a half without rows, and a row behind
+    // the last, stores nothing.
     if (half_on) {
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: 0; NaN stays
       const int64_t prow = (int64_t)(parts.first + z) * parts.rows + (int64_t)tok * a.Hq + h;
@@ -529,42 +546,54 @@ __global__ void __launch_bounds__(TC_NT, 1)
       // offset of this thread's row; -1: nothing to store
       const int64_t off = !real ? -1 : part ? (l == 0.f ? -1 : prow * D)
                                             : tok * a.o_ts + (int64_t)h * a.o_hs;
+      int64_t ro[8];  // of the rows that this lane stores a piece of
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
+      for (int e = 0; e < 8; ++e) ro[e] = __shfl_sync(0xffffffffu, off, 4 * e + (lane >> 3));
+      const uint32_t wr = ptx::smem_u32(rows) + lane * 128, rd = ptx::smem_u32(rows);
+#pragma unroll 1
+      for (int c = 0; c < D; c += 64) {  // 64 columns of E: 128 bytes a row; of fp32: twice
+        uint32_t o[64];
         ptx::tmem_ld_32x32b_x32(to + c, o);
+        ptx::tmem_ld_32x32b_x32(to + c + 32, o + 32);
         ptx::tmem_ld_wait();
         tc_regs(o);
+        tc_regs(o + 32);
         float* f = reinterpret_cast<float*>(o);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = l == 0.f ? 0.f : f[e] * inv;
-        if (part) {  // 32 columns of fp32: 128 bytes a row
+        for (int e = 0; e < 64; ++e) f[e] = l == 0.f ? 0.f : f[e] * inv;
+        if (!part) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<float4*>(rows + piece(lane, e)) =
-                make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-        } else {     // 64 columns
+            tc_sts(wr + ((e ^ (lane & 7)) << 4), Ty::pack(f[8 * e], f[8 * e + 1]),
+                   Ty::pack(f[8 * e + 2], f[8 * e + 3]), Ty::pack(f[8 * e + 4], f[8 * e + 5]),
+                   Ty::pack(f[8 * e + 6], f[8 * e + 7]));
+          __syncwarp();
+          E* const dst = reinterpret_cast<E*>(a.out) + c + 8 * (lane & 7);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint4*>(rows + piece(lane, (c & 32) / 8 + e)) = make_uint4(
-                Ty::pack(f[8 * e], f[8 * e + 1]), Ty::pack(f[8 * e + 2], f[8 * e + 3]),
-                Ty::pack(f[8 * e + 4], f[8 * e + 5]), Ty::pack(f[8 * e + 6], f[8 * e + 7]));
-          if ((c & 32) == 0) continue;
-        }
-        __syncwarp();
+          for (int e = 0; e < 8; ++e) {
+            const int row = 4 * e + (lane >> 3);
+            const uint4 v = tc_lds(rd + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+            if (ro[e] >= 0) *reinterpret_cast<uint4*>(dst + ro[e]) = v;
+          }
+          __syncwarp();
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {  // 8 lanes a row
-          const int row = 4 * e + (lane >> 3);
-          const int64_t ro = __shfl_sync(0xffffffffu, off, row);
-          const uint4 v = *reinterpret_cast<const uint4*>(rows + piece(row, lane & 7));
-          if (ro < 0) continue;
-          if (part)
-            *reinterpret_cast<uint4*>(parts.o + ro + c + 4 * (lane & 7)) = v;
-          else
-            *reinterpret_cast<uint4*>(reinterpret_cast<E*>(a.out) + ro + (c & ~63) +
-                                      8 * (lane & 7)) = v;
+          for (int q = 0; q < 2; ++q) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              tc_sts(wr + ((e ^ (lane & 7)) << 4), o[32 * q + 4 * e], o[32 * q + 4 * e + 1],
+                     o[32 * q + 4 * e + 2], o[32 * q + 4 * e + 3]);
+            __syncwarp();
+            float* const dst = parts.o + c + 32 * q + 4 * (lane & 7);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int row = 4 * e + (lane >> 3);
+              const uint4 v = tc_lds(rd + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+              if (ro[e] >= 0) *reinterpret_cast<uint4*>(dst + ro[e]) = v;
+            }
+            __syncwarp();
+          }
         }
-        __syncwarp();
       }
     }
   } else {
@@ -597,7 +626,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv, ++g_ring) {
         const int s = g_ring % L::ST;
-        tc_wait(bar_empty + 8 * s, ((uint32_t)(g_ring / L::ST) & 1u) ^ 1u, polls, abort_flag);
+        tc_wait(bar_empty + 8 * s, ((uint32_t)(g_ring / L::ST) & 1u) ^ 1u, tmo, abort_flag);
         if (*abort_flag) break;  // (no copy into a stage that is still in use)
         if (lane == 0) ptx::mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
         __syncwarp();
@@ -638,9 +667,10 @@ __global__ void __launch_bounds__(TC_NT, 1)
     const uint32_t tm_s = tm + L::COL_S + t * L::STEP_S, tm_p = tm + L::COL_P + t * 64,
                    tm_o = tm + L::COL_O + t * D;
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      uint32_t n = polls;
+      if (ptx::mbar_try_wait_now(bar, parity)) return;
+      const long long t0 = clock64();
       while (!ptx::mbar_try_wait_now(bar, parity)) {
-        if (*abort_flag || --n == 0) {
+        if (*abort_flag || clock64() - t0 > (long long)(tmo * 2ull)) {
           *abort_flag = 1;
           break;
         }
@@ -860,14 +890,27 @@ int64_t tc_tiles(int64_t T, int64_t R, int64_t G, bool ragged) {
   return T * G / TC_ROWS + (R < T ? R : T);
 }
 
-// Splits of the key axis: as many as give every SM a CTA, of at least two key
-// tiles each.
+// Splits of the key axis, where the CTAs would not fill the GPU: the number with the
+// least of rounds x (key tiles of a CTA + 3 for its start and end) plus the parts'
+// way through memory (a tile takes about 1.5 us, in which 9 MB pass) and, for
+// prompts, the joining kernel, which a decode step has anyway.
 int tc_splits(int64_t T, int64_t R, int Hq, int Hkv, int64_t keys, bool ragged, int sms) {
   const int64_t ctas = tc_tiles(T, R, Hq / Hkv, ragged) * Hkv;
-  int64_t s = sms / ctas;
-  const int64_t most = (keys + 2 * TC_KV - 1) / (2 * TC_KV);
-  s = s > most ? most : s;
-  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+  const int64_t nt = (keys + TC_KV - 1) / TC_KV;
+  const double part = (double)T * Hq * 128 * 8 / 9e6;
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 64 && s <= nt; ++s) {
+    const double rounds = (double)((ctas * s + sms - 1) / sms);
+    const double cost = rounds * (double)((nt + s - 1) / s + 3) +
+                        (s > 1 || !ragged ? s * part : 0) + (s > 1 && ragged ? 2 : 0);
+    if (s == 1 || cost < least) {
+      least = cost;
+      best = s;
+    }
+    if (s == 1 && ctas >= 4 * (int64_t)sms) break;
+  }
+  return best;
 }
 
 int launch_paged_tc(const PgAttnArgs& a, bool bf16, const PgParts& parts, int splits,

@@ -201,6 +201,22 @@ def test_prefill_attention(new, cached, hq, hkv, d, ps, dtype, layout):
     run_prefill(c, new, lens, d)
 
 
+@pytest.mark.parametrize("d,hq,hkv,dtype,ps", [
+    (128, 32, 4, BF16, 64), (64, 14, 2, F16, 16), (128, 8, 8, F16, 32), (64, 32, 32, BF16, 64),
+    (128, 16, 1, F16, 128)])
+def test_prefill_attention_many_requests(d, hq, hkv, dtype, ps):
+    """More tiles than the GPU has SMs, whole and half-filled ones in turn, and
+    requests without new tokens among them."""
+    rng = random.Random(d + hq)
+    R = 60 * 8 // hkv if hkv < 8 else 60
+    new = [rng.choice([1, 5, 16, 17, 40, 64, 100, 129, 0]) for _ in range(R)]
+    cached = [rng.choice([0, 0, 3, 127, 300]) for _ in range(R)]
+    c, lens = prefill_case(new, cached, hq, hkv, d, ps, dtype)
+    o = run_prefill(c, new, lens, d)
+    for _ in range(3):
+        assert torch.equal(run_prefill(c, new, lens, d), o)
+
+
 @pytest.mark.parametrize("cap,bias,bidir", [
     (30.0, False, None), (5.0, False, None), (0.0, True, None), (0.0, False, "mixed"),
     (50.0, True, None), (0.0, True, "mixed"), (20.0, True, "mixed")])
