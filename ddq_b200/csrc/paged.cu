@@ -58,8 +58,7 @@ int check_attn(const void* q, int64_t q_ts, int64_t q_hs, const void* out, int64
   if (!q || !out || !table || !lens) return DDQ_ERR_INVALID_ARGUMENT;
   if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.f)
     return DDQ_ERR_INVALID_ARGUMENT;
-  if (T > kIntMax || Hq < 1 || Hq > 1024 || Hq % Hkv != 0 || Hq / Hkv > 128 ||
-      T * Hq > kIntMax || table_width < 1 ||
+  if (T > kIntMax || Hq < 1 || Hq > 1024 || Hq % Hkv != 0 || T * Hq > kIntMax || table_width < 1 ||
       table_width > kIntMax || table_stride < table_width || q_ts < 0 || o_ts < 0 || q_hs < 0 ||
       o_hs < 0)
     return DDQ_ERR_SHAPE;
@@ -135,7 +134,7 @@ PgParts make_parts(void* ws, int64_t rows, int64_t D, int count) {
 }
 bool attn_shape(int64_t T, int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
                    int64_t page_size, int64_t prefix_len) {
-  return T > 0 && R > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 128 && D > 0 && table_width > 0 &&
+  return T > 0 && R > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && D > 0 && table_width > 0 &&
          page_size > 0 && prefix_len >= 0;
 }
 }  // namespace
@@ -190,7 +189,7 @@ extern "C" int ddq_paged_prefill_attention(
                block_table, table_stride, (int)table_width, lens, cu_new, bidir, prefix_pages,
                (int)prefix_len, slopes, scale, softcap, (int)T, (int)R, (int)Hq};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  st = launch_paged_tc(a, bf16, parts, splits, wait_timeout_ns(), s);
+  st = launch_paged_tc(a, bf16, parts, splits, wait_timeout_ns(), debug_flags(), s);
   if (st || splits == 1) return st;
   return launch_paged_merge(a, bf16, parts, s);
 }
@@ -220,5 +219,5 @@ extern "C" int ddq_paged_decode_attention(
                block_table, table_stride, (int)table_width, lens, nullptr, nullptr, prefix_pages,
                (int)prefix_len, slopes, scale, softcap, (int)B, (int)B, (int)Hq};
   return launch_paged_decode(a, cache->dtype == DDQ_DTYPE_BF16, workspace, plan,
-                             wait_timeout_ns(), reinterpret_cast<cudaStream_t>(stream));
+                             wait_timeout_ns(), debug_flags(), reinterpret_cast<cudaStream_t>(stream));
 }

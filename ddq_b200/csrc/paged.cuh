@@ -110,7 +110,7 @@ int launch_paged_rope_kv(const void* qkv, int64_t qkv_stride, const PgCache& c, 
                          int Hq, cudaStream_t s);
 int tc_splits(int64_t T, int64_t R, int Hq, int Hkv, int64_t keys, bool ragged, int sms);
 int launch_paged_tc(const PgAttnArgs& a, bool bf16, const PgParts& parts, int splits,
-                    unsigned long long tmo, cudaStream_t s);
+                    unsigned long long tmo, int debug_flags, cudaStream_t s);
 int pg_tensor_map(CUtensorMap* m, const PgCache& c, const void* base, bool bf16, int rows);
 // What a decode call runs and where its workspace holds what: the prefix parts
 // and the own part (as PgParts), then the side slots.
@@ -120,7 +120,7 @@ struct DcPlan {
 };
 DcPlan dc_plan(int64_t B, int Hq, int Hkv, int D, int64_t keys, int64_t prefix, int sms);
 int launch_paged_decode(const PgAttnArgs& a, bool bf16, void* ws, const DcPlan& plan,
-                        unsigned long long tmo, cudaStream_t s);
+                        unsigned long long tmo, int debug_flags, cudaStream_t s);
 int launch_paged_merge(const PgAttnArgs& a, bool bf16, const PgParts& parts, cudaStream_t s);
 
 }  // namespace ddq

@@ -51,7 +51,7 @@ struct DcSmem {
   unsigned long long full[DC_NW * DC_SLOTS];
   long long wsum[DC_NW];
   int most[DC_NW];
-  int start[DC_NW][4];
+  int start[DC_NW][6];
   int abort_flag;
 };
 
@@ -197,16 +197,19 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
     const long long u0 = (w0 + w) * uq + min(w0 + w, ur);
     long long at = (inc - sum) * segs;
     if (u0 < at || u0 >= inc * segs) continue;
-    int b = b0, n = units_of(pg_len(a, b));
+    int b = b0, len = pg_len(a, b), n = units_of(len);
     while (u0 >= at + (long long)n * segs) {
       at += (long long)n * segs;
-      n = units_of(pg_len(a, ++b));
+      len = pg_len(a, ++b);
+      n = units_of(len);
     }
     const int seg = (int)dc_div(u0 - at, n);
     sm.start[w][0] = b;
     sm.start[w][1] = seg / groups;
     sm.start[w][2] = seg % groups;
     sm.start[w][3] = (int)(u0 - at - (long long)seg * n);
+    sm.start[w][4] = len;
+    sm.start[w][5] = n;
   }
   __syncthreads();
   if (w0 + warp >= N) {
@@ -228,8 +231,8 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
     ++w.b;
     load_len(w);
   };
-  DcWalk cw{sm.start[warp][0], sm.start[warp][1], sm.start[warp][2], sm.start[warp][3], 0, 0};
-  load_len(cw);
+  DcWalk cw{sm.start[warp][0], sm.start[warp][1], sm.start[warp][2], sm.start[warp][3],
+            sm.start[warp][4], sm.start[warp][5]};
   const int count = (int)(uq + (worker < ur ? 1 : 0));
 
   // ---- loads: chunk after chunk of this warp, the page numbers one ahead
@@ -647,7 +650,7 @@ DcPlan dc_plan(int64_t B, int Hq, int Hkv, int D, int64_t keys, int64_t prefix, 
 }
 
 int launch_paged_decode(const PgAttnArgs& a, bool bf16, void* ws, const DcPlan& plan,
-                        unsigned long long tmo, cudaStream_t s) {
+                        unsigned long long tmo, int debug_flags, cudaStream_t s) {
   if (a.R > DC_MAXB) return DDQ_ERR_SHAPE;
   uint8_t* w = static_cast<uint8_t*>(ws);
   const int count = a.prefix_len ? plan.splits + 1 : 0;
@@ -659,7 +662,7 @@ int launch_paged_decode(const PgAttnArgs& a, bool bf16, void* ws, const DcPlan& 
                     reinterpret_cast<int2*>(w + plan.off_seg)};
   int st = DDQ_OK;
   if (count) {
-    st = launch_paged_tc(a, bf16, parts, plan.splits, tmo, s);
+    st = launch_paged_tc(a, bf16, parts, plan.splits, tmo, debug_flags, s);
     if (st) return st;
   }
   CUtensorMap tk, tv;

@@ -189,7 +189,8 @@ template <typename E, int D>
 __global__ void __launch_bounds__(TC_NT, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const PgAttnArgs a,
-                    const PgParts parts, const int splits, const unsigned long long tmo) {
+                    const PgParts parts, const int splits, const int skip_signal,
+                    const unsigned long long tmo) {
   using L = TcLayout<D>;
   using Ty = PgType<E>;
   constexpr bool ONE_S = L::ONE_S;
@@ -246,7 +247,38 @@ __global__ void __launch_bounds__(TC_NT, 1)
   // ---- the request and the tile of this CTA: requests and their tiles from the
   // last to the first, so that the CTAs that start last have the fewest keys
   int r = 0, tile = blockIdx.x, t_first = 0, n = a.T;
-  if (a.cu) {
+  int len = 0, most = 0;  // own keys, and the ones that bidir lets every row attend
+  if (a.cu && a.R <= 32) {  // each warp for itself: one round of loads, no barrier
+    const int rr = a.R - 1 - lane;
+    int c0 = 0, cn = 0, ln = 0, bd = 0;
+    if (rr >= 0) {
+      c0 = a.cu[rr];
+      cn = a.cu[rr + 1] - c0;
+      ln = a.lens[rr];
+      if (a.bidir) bd = a.bidir[rr];
+      if (c0 < 0 || c0 >= a.T || cn < 0) cn = 0;
+      cn = min(cn, a.T - c0);
+    }
+    const int tiles = (cn * G + TC_ROWS - 1) / TC_ROWS;
+    int s = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, tile < s && tile >= s - tiles);
+    if (hit == 0) {  // the grid covers the most tiles that T rows can make
+      if (warp == 9) ptx::tmem_dealloc(*tmem_holder, 512);
+      return;
+    }
+    const int src = __ffs(hit) - 1;
+    r = __shfl_sync(0xffffffffu, rr, src);
+    tile = __shfl_sync(0xffffffffu, s, src) - 1 - tile;
+    t_first = __shfl_sync(0xffffffffu, c0, src);
+    n = __shfl_sync(0xffffffffu, cn, src);
+    len = pg_clamp_len(a, __shfl_sync(0xffffffffu, ln, src));
+    most = __shfl_sync(0xffffffffu, bd, src);
+  } else if (a.cu) {
     int run = 0;
     for (int base = 0; base < a.R; base += TC_NT) {
       const int rr = a.R - 1 - (base + tid);
@@ -287,17 +319,18 @@ __global__ void __launch_bounds__(TC_NT, 1)
       if (found[0] >= 0) break;
     }
     r = found[0];
-    if (r < 0) {  // the grid covers the most tiles that T rows can make
+    if (r < 0) {
       if (warp == 9) ptx::tmem_dealloc(*tmem_holder, 512);
       return;
     }
     tile = found[1];
     t_first = found[2];
     n = found[3];
+    len = found[4];
+    most = found[5];
   }
   const int P = a.prefix_len;
-  const int len = a.cu ? found[4] : 0;
-  const int least = a.cu ? (a.bidir ? P + min(found[5], len) : 0) : P;
+  const int least = a.cu ? (a.bidir ? P + min(most, len) : 0) : P;
   const int row0 = tile * TC_ROWS, nrow = min(TC_ROWS, n * G - row0);
   const int halves = nrow > TC_HALF ? 2 : 1;
   // keys of the row of token i: those below end(i); the last row has the most
@@ -688,7 +721,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
       for (int e = 0; e < D / 16; ++e)
         ptx::mma_f16_ss_if(who, tm_s, dq + ((e >> 2) * L::HB + (e & 3) * 32) / 16,
                            b0 + ((e >> 2) * L::HB + (e & 3) * 32) / 16, id_qk, e != 0 ? 1u : 0u);
-      ptx::mma_commit_if(who, bar_s + 8 * t);
+      if (!skip_signal) ptx::mma_commit_if(who, bar_s + 8 * t);
       release(s);
     };
     wait(bar_q, 0);
@@ -914,7 +947,7 @@ int tc_splits(int64_t T, int64_t R, int Hq, int Hkv, int64_t keys, bool ragged, 
 }
 
 int launch_paged_tc(const PgAttnArgs& a, bool bf16, const PgParts& parts, int splits,
-                    unsigned long long tmo, cudaStream_t s) {
+                    unsigned long long tmo, int debug_flags, cudaStream_t s) {
   const int G = a.Hq / a.c.Hkv;
   const int64_t tiles = tc_tiles(a.T, a.R, G, a.cu != nullptr);
   if (tiles > 0x7fffffff || a.c.Hkv > 65535) return DDQ_ERR_SHAPE;
@@ -939,7 +972,9 @@ int launch_paged_tc(const PgAttnArgs& a, bool bf16, const PgParts& parts, int sp
     const int ast = ensure_smem_attr(once, dev, kern, smem);
     if (ast) return ast;
     cfg.dynamicSmemBytes = smem;
-    e = cudaLaunchKernelEx(&cfg, kern, tk, tv, a, parts, splits, tmo);
+    // test hook (ddq_set_debug bit 0): no scores-ready signal, so that the softmax's
+    // bounded waits run out and every role winds down
+    e = cudaLaunchKernelEx(&cfg, kern, tk, tv, a, parts, splits, debug_flags & 1, tmo);
     return DDQ_OK;
   };
   if (a.c.D == 64)

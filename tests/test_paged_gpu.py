@@ -424,6 +424,52 @@ def test_a_length_beyond_the_table_is_reported():
     assert device_error() == ERR_PAGE
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(d):
+    """The scores-ready signal left out (a test hook): the bounded waits give up, the
+    kernel winds down, and the device error word says so."""
+    from ddq_b200 import _lib, paged
+    new, cached = [300, 20], [100, 0]
+    c, lens = prefill_case(new, cached, 8, 2, d, 16, F16)
+    lib = _lib.load()
+    assert lib.ddq_set_debug(1, 2_000_000) == 0          # 2 ms
+    try:
+        paged.prefill_attention(c["q"], c["kp"], c["vp"], c["table"], c["cu"], c["lens"],
+                                d ** -0.5)
+        torch.cuda.synchronize()
+    finally:
+        lib.ddq_set_debug(0, 0)
+    assert device_error() == 7                            # DDQ_ERR_TIMEOUT
+    run_prefill(c, new, lens, d)
+
+
+def test_pages_far_into_a_large_pool():
+    """Offsets of the pool beyond 2^32 bytes and 2^31 elements."""
+    from ddq_b200 import paged
+    hq, hkv, d, ps, P = 16, 8, 128, 64, 36000            # 2.4 G elements each
+    kp = torch.empty(P, hkv, ps, d, dtype=F16, device="cuda")
+    vp = torch.empty_like(kp)
+    gen = torch.Generator().manual_seed(2)
+    pages = torch.tensor([P - 1, 1, P - 7, P - 2, 33000, 5], dtype=torch.int32)
+    n = 300
+    slots = (pages.long()[torch.arange(n) // ps] * ps + torch.arange(n) % ps).cuda()
+    cos, sin = ref.rope_tables(n, d)
+    qkv = torch.randn(n, (hq + 2 * hkv) * d, generator=gen).half().cuda()
+    pos = torch.arange(n, device="cuda")
+    q = paged.rope_kv_write(qkv, kp, vp, cos, sin, slots, pos, hq, hkv, d)
+    y = ref.rope_reference(qkv[:, :(hq + hkv) * d].reshape(n, -1, d), cos, sin)
+    k, v = y[:, hq:], qkv[:, (hq + hkv) * d:].reshape(n, hkv, d)
+    assert torch.equal(kp[slots // ps, :, slots % ps], k)
+    assert torch.equal(vp[slots // ps, :, slots % ps], v)
+    table = pages[None].cuda()
+    o = paged.prefill_attention(q, kp, vp, table, ints([0, n]), ints([n]), d ** -0.5)
+    want, tol = ref.prefill_reference(q, kp, vp, table, [n], [n], d ** -0.5, 0.0, None, None)
+    close(o, want, tol)
+    o = paged.decode_attention(q[-1:], kp, vp, table[:, 2:], ints([n - 2 * ps]), d ** -0.5,
+                               prefix_pages=table[0, :2].contiguous(), prefix_len=2 * ps)
+    close(o[0], want[-1], tol[-1])
+
+
 def test_results_do_not_change_from_call_to_call():
     lens, prefix = [700, 3, 64, 2000], 900
     c = decode_case(lens, prefix, 14, 2, 64, 16, F16)
