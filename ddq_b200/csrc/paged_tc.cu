@@ -29,10 +29,12 @@
 // rescaled: after the first tiles a row's maximum hardly grows.
 //
 // Warps 0-3 and 4-7: softmax of half 0 and 1.  Warp 8: TMA, one box per page
-// and 64 dimensions, each lane its own.  Warps 9 and 10: MMA issue, a half each.  While one half is
-// in its softmax the tensor core works for the other.  64-wide heads leave TMEM
-// for P beside S, so S of the next tile is made during the softmax of this one;
-// with 128-wide heads P takes S's place and it follows PV.
+// and 64 dimensions, each lane its own.  Warps 9 and 10: MMA issue, a half each.
+// S, one for both halves in turn, is free as soon as its rows are in registers, so
+// the next scores are made during the softmax, and the halves stay half a tile
+// apart: while one uses the special-function pipe, the other loads and stores (with
+// an S each they ran in step: 97.7 us instead of 93.0 for 509 tokens behind 32259
+// keys, 64-wide heads).
 #include <cudaTypedefs.h>
 
 #include <mutex>
@@ -62,11 +64,8 @@ struct TcLayout {
   static constexpr int OFF_RING = 2 * TILE;
   static constexpr int OFF_BAR = OFF_RING + ST * TILE;
   static constexpr int SMEM = OFF_BAR + 512 + 1024;
-  // TMEM columns: scores (64-wide heads: of each half; 128-wide ones: of both in
-  // turn), weights and outputs of each half
-  static constexpr bool ONE_S = D == 128;
-  static constexpr int COL_S = 0, STEP_S = ONE_S ? 0 : 128;
-  static constexpr int COL_P = ONE_S ? 128 : 256, COL_O = COL_P + 128;
+  // TMEM columns: scores (of both halves in turn), weights and outputs of each half
+  static constexpr int COL_S = 0, COL_P = 128, COL_O = 256;
 };
 
 __device__ __forceinline__ float tc_exp2(float x) {
@@ -114,6 +113,7 @@ __device__ __forceinline__ TcF2 tc_pk(float a, float b) {
   asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ TcF2 tc_pk1(float a) { return tc_pk(a, a); }
 __device__ __forceinline__ void tc_un(TcF2 x, float& a, float& b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
 }
@@ -185,7 +185,9 @@ __device__ __forceinline__ float tc_max3(float a, float b, float c) {
   return y;
 }
 
-template <typename E, int D>
+// SCORED: scores that are capped or biased, or whose scale is not positive; the
+// plain kernel has none of that code.
+template <typename E, int D, bool SCORED>
 __global__ void __launch_bounds__(TC_NT, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const PgAttnArgs a,
@@ -193,7 +195,6 @@ __global__ void __launch_bounds__(TC_NT, 1)
                     const unsigned long long tmo) {
   using L = TcLayout<D>;
   using Ty = PgType<E>;
-  constexpr bool ONE_S = L::ONE_S;
   extern __shared__ uint8_t tc_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -408,14 +409,40 @@ __global__ void __launch_bounds__(TC_NT, 1)
       tc_arrive(bar_q, lane);
     }
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + L::COL_S + t * L::STEP_S + lanes;
+    const uint32_t ts = tmem + L::COL_S + lanes;
     const uint32_t tp = tmem + L::COL_P + t * 64 + lanes;
     const uint32_t to = tmem + L::COL_O + t * D + lanes;
     if (half_on) {
       constexpr float LOG2E = 1.4426950408889634f;
-      const bool plain = a.cap == 0.f && a.slopes == nullptr && a.scale > 0.f;
-      const float mul = plain ? a.scale * LOG2E : 1.f;
-      const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.f;
+      const float kk = a.scale * LOG2E, mul = SCORED ? 1.f : kk;
+      const float slope = SCORED && a.slopes ? a.slopes[h] * LOG2E : 0.f;
+      const float r2 = SCORED && a.cap > 0.f ? (a.scale / a.cap) * (a.scale / a.cap) : 0.f;
+      const float r8 = (r2 * r2) * (r2 * r2);
+      const TcF2 cap0 = tc_pk1(a.cap > 0.f ? kk * 0.999999987f : kk),
+                 cap1 = tc_pk1(kk * -0.333330694f * r2),
+                 cap2 = tc_pk1(kk * 0.133247793f * (r2 * r2)),
+                 cap3 = tc_pk1(kk * -0.0529860753f * (r2 * r2 * r2)),
+                 cap4 = tc_pk1(kk * 0.0171350066f * r8);
+      // |y| <= 1/2, y = scale s / cap: cap tanh(y) = scale s P(y^2), P the minimax
+      // polynomial of degree 4 of tanh(sqrt u) / sqrt(u) on [0, 1/4] (Remez, error
+      // 2^-26), its coefficients in powers of s^2: seven packed operations for two
+      // biased scores, no special function.  Without a cap P is 1.
+      auto capped_poly = [&](TcF2 x) {
+        const TcF2 v = tc_mul2(x, x);
+        return tc_fma2(v, tc_fma2(v, tc_fma2(v, tc_fma2(v, cap4, cap3), cap2), cap1), cap0);
+      };
+      auto capped = [&](float s0, float s1) {
+        const TcF2 x = tc_pk(s0, s1);
+        return tc_mul2(x, capped_poly(x));
+      };
+      auto capped_add = [&](float s0, float s1, TcF2 b) {
+        const TcF2 x = tc_pk(s0, s1);
+        return tc_fma2(x, capped_poly(x), b);
+      };
+      // the largest score for that polynomial; its powers and coefficients are finite
+      const float poly_max = !(kk * r8 < 1e30f && kk * r8 > -1e30f) ? -1.f
+                             : a.cap > 0.f ? fminf(0.5f * a.cap / fabsf(a.scale), 1e18f)
+                                           : 1e18f;
       for (int k = 0; k < cnt; ++k) {
         const int j0 = key0(k);
         const int lim = min(end, limit(k)) - j0;  // keys of this tile that the row attends
@@ -425,61 +452,78 @@ __global__ void __launch_bounds__(TC_NT, 1)
         // the row into registers, and S is free for the next scores
         uint32_t u[128];
         float* s = reinterpret_cast<float*>(u);
+        auto load_row = [&]() {
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) ptx::tmem_ld_32x32b_x32(ts + c, u + c);
-        ptx::tmem_ld_wait();
+          for (int c = 0; c < 128; c += 32) ptx::tmem_ld_32x32b_x32(ts + c, u + c);
+          ptx::tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) tc_regs(u + c);
+          for (int c = 0; c < 128; c += 32) tc_regs(u + c);
+        };
+        load_row();
+        bool poly = false;
+        if constexpr (SCORED) {
+          // to log2 units, capped and biased.  Where the polynomial serves all scores of
+          // the warp: in registers, below.  Otherwise 32 scores at a time and back to S,
+          // so that this rarer code, with more of its values alive, does not take
+          // registers from the rest (all in registers it spilled: 202 us instead of 180
+          // for 7679 tokens of 12 packed documents, 128-wide heads).
+          const float d0 = (float)(pos - j0);
+          float big = 0.f;
+#pragma unroll
+          for (int c = 0; c < 128; c += 2) big = tc_max3(big, fabsf(s[c]), fabsf(s[c + 1]));
+          poly = __all_sync(0xffffffffu, big <= poly_max);
+          if (!poly) {
+            const float k2 = a.cap > 0.f ? 2.f * kk / a.cap : 0.f, A = a.cap * LOG2E;
+#pragma unroll 1
+            for (int c0 = 0; c0 < TC_KV; c0 += 32) {
+              uint32_t o[32];
+              ptx::tmem_ld_32x32b_x32(ts + c0, o);
+              ptx::tmem_ld_wait();
+              tc_regs(o);
+              float* x = reinterpret_cast<float*>(o);
+              const float dc = d0 - (float)c0;
+              if (a.cap > 0.f) {
+                // cap tanh(y) = cap - 2 cap / (exp(2 y) + 1): an absolute error of a
+                // few 2^-23 cap, also where the exponential overflows
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                  x[c] = fmaf(-2.f * A, tc_rcp(tc_exp2(x[c] * k2) + 1.f), A);
+              } else {
+#pragma unroll
+                for (int c = 0; c < 32; ++c) x[c] *= kk;
+              }
+              if (a.slopes) {
+#pragma unroll
+                for (int c = 0; c < 32; ++c) x[c] = fmaf(-slope, fabsf(dc - (float)c), x[c]);
+              }
+              ptx::tmem_st_32x32b_x32(ts + c0, o);
+            }
+            ptx::tmem_st_wait();
+            load_row();
+          }
+        }
         ptx::tc_fence_before();
         tc_arrive(bar_sfree + 8 * t, lane);
-        if (!plain) {  // to log2 units, capped and biased
-          if (a.cap > 0.f) {
-            float big = 0.f;
-#pragma unroll
-            for (int c = 0; c < 128; c += 2) big = tc_max3(big, fabsf(s[c]), fabsf(s[c + 1]));
-            if (__all_sync(0xffffffffu, big * fabsf(a.scale) <= 0.5f * a.cap)) {
-              // |y| <= 1/2, y = scale s / cap: cap tanh(y) = scale s P(y^2), P the
-              // minimax polynomial of degree 4 of tanh(sqrt u) / sqrt(u) on [0, 1/4]
-              // (Remez, error 2^-26), its coefficients in powers of s^2: six packed
-              // operations for two scores, no special function
-              const float kk = a.scale * LOG2E, r2 = (a.scale / a.cap) * (a.scale / a.cap);
-              const float cap0 = kk * 0.999999987f, cap1 = kk * -0.333330694f * r2,
-                          cap2 = kk * 0.133247793f * (r2 * r2),
-                          cap3 = kk * -0.0529860753f * (r2 * r2 * r2),
-                          cap4 = kk * 0.0171350066f * (r2 * r2) * (r2 * r2);
+        if constexpr (SCORED) {
+          if (poly) {
+            // no key of the tile behind a row: the bias is slope c - slope d0
+            if (__all_sync(0xffffffffu, a.slopes == nullptr || pos - j0 >= TC_KV - 1)) {
+              const TcF2 sl2 = tc_pk1(slope), base = tc_pk1(-slope * (float)(pos - j0));
 #pragma unroll
               for (int c = 0; c < 128; c += 2) {
-                const TcF2 x = tc_pk(s[c], s[c + 1]), v = tc_mul2(x, x);
-                TcF2 q = tc_fma2(v, tc_pk(cap4, cap4), tc_pk(cap3, cap3));
-                q = tc_fma2(v, q, tc_pk(cap2, cap2));
-                q = tc_fma2(v, q, tc_pk(cap1, cap1));
-                q = tc_fma2(v, q, tc_pk(cap0, cap0));
-                tc_un(tc_mul2(x, q), s[c], s[c + 1]);
+                const TcF2 b = tc_fma2(sl2, tc_pk((float)c, (float)(c + 1)), base);
+                tc_un(capped_add(s[c], s[c + 1], b), s[c], s[c + 1]);
               }
             } else {
-              // cap tanh(y) = cap - 2 cap / (exp(2 y) + 1): an absolute error of a
-              // few 2^-23 cap, also where the exponential overflows
-              const float kk = 2.f * LOG2E * a.scale / a.cap, A = a.cap * LOG2E;
+              const TcF2 d2 = tc_pk1((float)(pos - j0));
 #pragma unroll
-              for (int c = 0; c < 128; ++c)
-                s[c] = fmaf(-2.f * A, tc_rcp(tc_exp2(s[c] * kk) + 1.f), A);
-            }
-          } else {
-            const float kk = a.scale * LOG2E;
-#pragma unroll
-            for (int c = 0; c < 128; ++c) s[c] *= kk;
-          }
-          if (a.slopes) {
-            const float d0 = (float)(pos - j0);
-            const TcF2 d2 = tc_pk(d0, d0), sl2 = tc_pk(-slope, -slope);
-            if (__all_sync(0xffffffffu, pos - j0 >= TC_KV - 1)) {  // no key behind the row
-#pragma unroll
-              for (int c = 0; c < 128; c += 2)
-                tc_un(tc_fma2(sl2, tc_add2(d2, tc_pk((float)-c, (float)(-c - 1))),
-                              tc_pk(s[c], s[c + 1])), s[c], s[c + 1]);
-            } else {
-#pragma unroll
-              for (int c = 0; c < 128; ++c) s[c] = fmaf(-slope, fabsf(d0 - (float)c), s[c]);
+              for (int c = 0; c < 128; c += 2) {
+                float t0, t1;
+                tc_un(tc_add2(d2, tc_pk((float)-c, (float)(-c - 1))), t0, t1);
+                tc_un(capped(s[c], s[c + 1]), s[c], s[c + 1]);
+                s[c] = fmaf(-slope, fabsf(t0), s[c]);
+                s[c + 1] = fmaf(-slope, fabsf(t1), s[c + 1]);
+              }
             }
           }
         }
@@ -548,7 +592,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
         };
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          if (full && plain) weights(hf, std::true_type()); else weights(hf, std::false_type());
+          if (full) weights(hf, std::true_type()); else weights(hf, std::false_type());
           if (hf == 0 && k > 0) {  // P of the tile before has been read
             tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
             ptx::tc_fence_after();
@@ -697,7 +741,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
     const uint64_t dq = ptx::smem_desc_sw128(sbase + t * L::TILE);
     const uint64_t dk = ptx::smem_desc_sw128(sbase + L::OFF_RING);
     const uint64_t dv = ptx::smem_desc_sw128_mn(sbase + L::OFF_RING, L::HB);
-    const uint32_t tm_s = tm + L::COL_S + t * L::STEP_S, tm_p = tm + L::COL_P + t * 64,
+    const uint32_t tm_s = tm + L::COL_S, tm_p = tm + L::COL_P + t * 64,
                    tm_o = tm + L::COL_O + t * D;
     auto wait = [&](uint32_t bar, uint32_t parity) {
       if (ptx::mbar_try_wait_now(bar, parity)) return;
@@ -727,7 +771,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
     wait(bar_q, 0);
     wait(bar_full, 0);
     // half 1's first scores go where half 0's were, once those have been read
-    if (ONE_S && t == 1) {
+    if (t == 1) {
       wait(bar_sfree, 0);
       ptx::tc_fence_after();
     }
@@ -752,12 +796,12 @@ __global__ void __launch_bounds__(TC_NT, 1)
       }
       if (k + 1 < cnt_u) {
         wait(bar_full + 8 * sk, phk);
-        // S is free once it has been read: by its own half, or, where both share
-        // it, by the other one (half 1 of this tile; half 0 of the next)
-        if (ONE_S && halves_u == 2)
+        // S is free once the other half has read it (half 1 of this tile; half 0 of
+        // the next), or this one where there is no other
+        if (halves_u == 2)
           wait(bar_sfree + 8 * (1 - t), t == 0 ? par : par ^ 1u);
         else
-          wait(bar_sfree + 8 * t, par);
+          wait(bar_sfree, par);
         ptx::tc_fence_after();
         qk(sk);
       }
@@ -957,7 +1001,8 @@ int launch_paged_tc(const PgAttnArgs& a, bool bf16, const PgParts& parts, int sp
   if (!st) st = pg_tensor_map(&tv, a.c, a.c.v, bf16, br);
   if (st) return st;
   const int dev = current_device();
-  static SmemAttrOnce attr[2][2];
+  static SmemAttrOnce attr[2][2][2];
+  const bool scored = a.cap > 0.f || a.slopes != nullptr || !(a.scale > 0.f);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)tiles, (unsigned)a.c.Hkv, (unsigned)splits);
   cfg.blockDim = dim3(TC_NT);
@@ -977,12 +1022,14 @@ int launch_paged_tc(const PgAttnArgs& a, bool bf16, const PgParts& parts, int sp
     e = cudaLaunchKernelEx(&cfg, kern, tk, tv, a, parts, splits, debug_flags & 1, tmo);
     return DDQ_OK;
   };
+#define DDQ_TC(E_, D_, B_)                                                                      \
+  (scored ? go(paged_tc_kernel<E_, D_, true>, attr[D_ / 128][B_][1], TcLayout<D_>::SMEM)        \
+          : go(paged_tc_kernel<E_, D_, false>, attr[D_ / 128][B_][0], TcLayout<D_>::SMEM))
   if (a.c.D == 64)
-    st = bf16 ? go(paged_tc_kernel<__nv_bfloat16, 64>, attr[0][1], TcLayout<64>::SMEM)
-              : go(paged_tc_kernel<__half, 64>, attr[0][0], TcLayout<64>::SMEM);
+    st = bf16 ? DDQ_TC(__nv_bfloat16, 64, 1) : DDQ_TC(__half, 64, 0);
   else
-    st = bf16 ? go(paged_tc_kernel<__nv_bfloat16, 128>, attr[1][1], TcLayout<128>::SMEM)
-              : go(paged_tc_kernel<__half, 128>, attr[1][0], TcLayout<128>::SMEM);
+    st = bf16 ? DDQ_TC(__nv_bfloat16, 128, 1) : DDQ_TC(__half, 128, 0);
+#undef DDQ_TC
   if (st) return st;
   if (e != cudaSuccess) {
     cudaGetLastError();
