@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
   const uint32_t sbase = ptx::smem_u32(smem);
   __shared__ int found[6], wsum[TC_NT / 32];  // request, tile, first row, rows, keys, bidir
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int G = a.Hq / a.c.Hkv, g = blockIdx.y, z = blockIdx.z;
+  const int G = a.Hq / a.c.Hkv, g = blockIdx.x % a.c.Hkv, z = blockIdx.y;
 
   const uint32_t bar_full = sbase + L::OFF_BAR;
   const uint32_t bar_empty = bar_full + 8 * L::ST;
@@ -245,9 +245,12 @@ __global__ void __launch_bounds__(TC_NT, 1)
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
 
-  // ---- the request and the tile of this CTA: requests and their tiles from the
-  // last to the first, so that the CTAs that start last have the fewest keys
-  int r = 0, tile = blockIdx.x, t_first = 0, n = a.T;
+  // ---- the request and the tile of this CTA, kv heads next to each other: the CTAs
+  // that start last shall have the fewest keys, so the tiles of a request go from the
+  // last to the first and of up to 32 requests the longest is first (7679 tokens of 12
+  // documents: 120 us; in the order of the batch 128, a head after the other 154; four
+  // prompts of 4096 tokens: 504, a head after the other 514)
+  int r = 0, tile = blockIdx.x / a.c.Hkv, t_first = 0, n = a.T;
   int len = 0, most = 0;  // own keys, and the ones that bidir lets every row attend
   if (a.cu && a.R <= 32) {  // each warp for itself: one round of loads, no barrier
     const int rr = a.R - 1 - lane;
@@ -261,11 +264,10 @@ __global__ void __launch_bounds__(TC_NT, 1)
       cn = min(cn, a.T - c0);
     }
     const int tiles = (cn * G + TC_ROWS - 1) / TC_ROWS;
-    int s = tiles;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
+    int s = 0;
+    for (int e = 0; e < a.R; ++e) {
+      const int le = __shfl_sync(0xffffffffu, ln, e), te = __shfl_sync(0xffffffffu, tiles, e);
+      if (le > ln || (le == ln && e <= lane)) s += te;
     }
     const uint32_t hit = __ballot_sync(0xffffffffu, tile < s && tile >= s - tiles);
     if (hit == 0) {  // the grid covers the most tiles that T rows can make
@@ -425,8 +427,9 @@ __global__ void __launch_bounds__(TC_NT, 1)
                  cap4 = tc_pk1(kk * 0.0171350066f * r8);
       // |y| <= 1/2, y = scale s / cap: cap tanh(y) = scale s P(y^2), P the minimax
       // polynomial of degree 4 of tanh(sqrt u) / sqrt(u) on [0, 1/4] (Remez, error
-      // 2^-26), its coefficients in powers of s^2: seven packed operations for two
-      // biased scores, no special function.  Without a cap P is 1.
+      // 2^-26), its coefficients in powers of s^2; up to |y| = 1/6 of degree 2 (error
+      // 2^-24.7): six or four packed operations for two scores, their bias added, and no
+      // special function.  Without a cap P is 1.
       auto capped_poly = [&](TcF2 x) {
         const TcF2 v = tc_mul2(x, x);
         return tc_fma2(v, tc_fma2(v, tc_fma2(v, tc_fma2(v, cap4, cap3), cap2), cap1), cap0);
@@ -439,10 +442,14 @@ __global__ void __launch_bounds__(TC_NT, 1)
         const TcF2 x = tc_pk(s0, s1);
         return tc_fma2(x, capped_poly(x), b);
       };
-      // the largest score for that polynomial; its powers and coefficients are finite
+      // the largest scores for the polynomials; their powers and coefficients are finite
       const float poly_max = !(kk * r8 < 1e30f && kk * r8 > -1e30f) ? -1.f
                              : a.cap > 0.f ? fminf(0.5f * a.cap / fabsf(a.scale), 1e18f)
                                            : 1e18f;
+      const TcF2 low0 = tc_pk1(a.cap > 0.f ? kk * 0.999999965f : kk),
+                 low1 = tc_pk1(kk * -0.333310343f * r2),
+                 low2 = tc_pk1(kk * 0.131114860f * (r2 * r2));
+      const float poly2_max = a.cap > 0.f ? poly_max * (1.f / 3) : poly_max;
       for (int k = 0; k < cnt; ++k) {
         const int j0 = key0(k);
         const int lim = min(end, limit(k)) - j0;  // keys of this tile that the row attends
@@ -461,6 +468,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
         };
         load_row();
         bool poly = false;
+        float step = 0.f, big = 0.f;
         if constexpr (SCORED) {
           // to log2 units, capped and biased.  Where the polynomial serves all scores of
           // the warp: in registers, below.  Otherwise 32 scores at a time and back to S,
@@ -468,7 +476,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
           // registers from the rest (all in registers it spilled: 202 us instead of 180
           // for 7679 tokens of 12 packed documents, 128-wide heads).
           const float d0 = (float)(pos - j0);
-          float big = 0.f;
+          big = 0.f;
 #pragma unroll
           for (int c = 0; c < 128; c += 2) big = tc_max3(big, fabsf(s[c]), fabsf(s[c + 1]));
           poly = __all_sync(0xffffffffu, big <= poly_max);
@@ -506,13 +514,28 @@ __global__ void __launch_bounds__(TC_NT, 1)
         tc_arrive(bar_sfree + 8 * t, lane);
         if constexpr (SCORED) {
           if (poly) {
-            // no key of the tile behind a row: the bias is slope c - slope d0
-            if (__all_sync(0xffffffffu, a.slopes == nullptr || pos - j0 >= TC_KV - 1)) {
-              const TcF2 sl2 = tc_pk1(slope), base = tc_pk1(-slope * (float)(pos - j0));
+            // no key of the tile behind a row, or all: the bias is linear, in groups of
+            // eight keys the same up to a step that the maximum and the exponent add
+            const bool behind = __all_sync(0xffffffffu, pos <= j0);
+            if (behind ||
+                __all_sync(0xffffffffu, a.slopes == nullptr || pos - j0 >= TC_KV - 1)) {
+              const float sl = behind ? -slope : slope, base = -sl * (float)(pos - j0);
+              TcF2 b[4];
 #pragma unroll
-              for (int c = 0; c < 128; c += 2) {
-                const TcF2 b = tc_fma2(sl2, tc_pk((float)c, (float)(c + 1)), base);
-                tc_un(capped_add(s[c], s[c + 1], b), s[c], s[c + 1]);
+              for (int e = 0; e < 4; ++e)
+                b[e] = tc_pk(fmaf(sl, (float)(2 * e), base), fmaf(sl, (float)(2 * e + 1), base));
+              step = 8.f * sl;
+              if (__all_sync(0xffffffffu, big <= poly2_max)) {
+#pragma unroll
+                for (int c = 0; c < 128; c += 2) {
+                  const TcF2 x = tc_pk(s[c], s[c + 1]), v = tc_mul2(x, x);
+                  const TcF2 q = tc_fma2(v, tc_fma2(v, low2, low1), low0);
+                  tc_un(tc_fma2(x, q, b[(c >> 1) & 3]), s[c], s[c + 1]);
+                }
+              } else {
+#pragma unroll
+                for (int c = 0; c < 128; c += 2)
+                  tc_un(capped_add(s[c], s[c + 1], b[(c >> 1) & 3]), s[c], s[c + 1]);
               }
             } else {
               const TcF2 d2 = tc_pk1((float)(pos - j0));
@@ -532,17 +555,31 @@ __global__ void __launch_bounds__(TC_NT, 1)
           for (int c = 0; c < 128; ++c)
             if (c >= lim) s[c] = -INFINITY;
         }
-        float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
+        float mx;
+        if constexpr (SCORED) {
+          float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-        for (int c = 4; c < 124; c += 8) {
-          x0 = tc_max3(x0, s[c], s[c + 1]);
-          x1 = tc_max3(x1, s[c + 2], s[c + 3]);
-          x2 = tc_max3(x2, s[c + 4], s[c + 5]);
-          x3 = tc_max3(x3, s[c + 6], s[c + 7]);
+          for (int c = 0; c < 128; c += 8) {
+            float y = tc_max3(s[c], s[c + 1], s[c + 2]);
+            y = tc_max3(y, s[c + 3], s[c + 4]);
+            const float w = tc_max3(s[c + 5], s[c + 6], s[c + 7]);
+            y = fmaxf(y, w) + step * (float)(c / 8);
+            if (c & 8) x0 = fmaxf(x0, y); else x1 = fmaxf(x1, y);
+          }
+          mx = fmaxf(x0, x1);
+        } else {
+          float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
+#pragma unroll
+          for (int c = 4; c < 124; c += 8) {
+            x0 = tc_max3(x0, s[c], s[c + 1]);
+            x1 = tc_max3(x1, s[c + 2], s[c + 3]);
+            x2 = tc_max3(x2, s[c + 4], s[c + 5]);
+            x3 = tc_max3(x3, s[c + 6], s[c + 7]);
+          }
+          x0 = tc_max3(x0, s[124], s[125]);
+          x1 = tc_max3(x1, s[126], s[127]);
+          mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * mul;
         }
-        x0 = tc_max3(x0, s[124], s[125]);
-        x1 = tc_max3(x1, s[126], s[127]);
-        const float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * mul;
         if (__any_sync(0xffffffffu, mx > m + TC_LAZY)) {
           float alpha = 1.f;
           if (mx > m + TC_LAZY) {  // also the first keys of the row (m = -inf)
@@ -575,11 +612,17 @@ __global__ void __launch_bounds__(TC_NT, 1)
 #pragma unroll
           for (int c = 64 * hf; c < 64 * hf + 64; c += 2) {
             float y0, y1;
-            tc_un(tc_fma2(tc_pk(s[c], s[c + 1]), mul2, mu2), y0, y1);
+            if constexpr (SCORED)
+              tc_un(tc_add2(tc_pk(s[c], s[c + 1]), tc_pk1(fmaf(step, (float)(c / 8), -mu))),
+                    y0, y1);
+            else
+              tc_un(tc_fma2(tc_pk(s[c], s[c + 1]), mul2, mu2), y0, y1);
             // one pair of four on the FMA pipe: the special-function pipe, 16
             // results a cycle and SM, is the narrower one (four prompts of 4096
             // tokens, 128-wide heads: none 597 us, 1/8 570, 1/4 561, 3/8 563;
-            // where keys are masked all on the latter, for weights of exactly 0)
+            // where keys are masked all on the latter, for weights of exactly 0; capped
+            // or biased scores use the FMA pipe enough, 154 us for the documents above
+            // instead of 166)
             if (decltype(poly)::value && (c & 6) == 4) {
               tc_un(tc_poly_exp2(y0, y1), y0, y1);
             } else {
@@ -592,7 +635,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
         };
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          if (full) weights(hf, std::true_type()); else weights(hf, std::false_type());
+          if (full && !SCORED) weights(hf, std::true_type()); else weights(hf, std::false_type());
           if (hf == 0 && k > 0) {  // P of the tile before has been read
             tc_wait(bar_pv + 8 * t, (uint32_t)(k - 1) & 1u, tmo, abort_flag);
             ptx::tc_fence_after();
@@ -994,7 +1037,7 @@ int launch_paged_tc(const PgAttnArgs& a, bool bf16, const PgParts& parts, int sp
                     unsigned long long tmo, int debug_flags, cudaStream_t s) {
   const int G = a.Hq / a.c.Hkv;
   const int64_t tiles = tc_tiles(a.T, a.R, G, a.cu != nullptr);
-  if (tiles > 0x7fffffff || a.c.Hkv > 65535) return DDQ_ERR_SHAPE;
+  if (tiles > 0x7fffffff / a.c.Hkv) return DDQ_ERR_SHAPE;
   CUtensorMap tk, tv;
   const int br = (1 << a.c.page_shift) < TC_KV ? (1 << a.c.page_shift) : TC_KV;
   int st = pg_tensor_map(&tk, a.c, a.c.k, bf16, br);
@@ -1004,7 +1047,7 @@ int launch_paged_tc(const PgAttnArgs& a, bool bf16, const PgParts& parts, int sp
   static SmemAttrOnce attr[2][2][2];
   const bool scored = a.cap > 0.f || a.slopes != nullptr || !(a.scale > 0.f);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)tiles, (unsigned)a.c.Hkv, (unsigned)splits);
+  cfg.gridDim = dim3((unsigned)(tiles * a.c.Hkv), (unsigned)splits);
   cfg.blockDim = dim3(TC_NT);
   cfg.stream = s;
   cudaLaunchAttribute at;

@@ -172,9 +172,9 @@ def prefill_case(new, cached, hq, hkv, d, ps, dtype, layout="hnd", cap=0.0, bias
                 bidir=ints(bidir) if bidir is not None else None), lens
 
 
-def run_prefill(c, new, lens, d, cap=0.0, bidir=None, out=None, prefix=0):
+def run_prefill(c, new, lens, d, cap=0.0, bidir=None, out=None, prefix=0, scale=None):
     from ddq_b200 import paged
-    scale = d ** -0.5
+    scale = d ** -0.5 if scale is None else scale
     o = paged.prefill_attention(c["q"], c["kp"], c["vp"], c["table"], c["cu"], c["lens"], scale,
                                 softcap=cap, slopes=c["slopes"], bidir=c["bidir"], out=out,
                                 prefix_pages=c["prefix"], prefix_len=prefix)
@@ -226,6 +226,36 @@ def test_prefill_attention_masks_and_scores(cap, bias, bidir, d, dtype, hq, hkv)
     bd = [100, 301, 9999, 0, -5] if bidir else None
     c, lens = prefill_case(new, cached, hq, hkv, d, 32, dtype, "hnd", cap, bias, bd, qscale=2.0)
     run_prefill(c, new, lens, d, cap, bd)
+
+
+@pytest.mark.parametrize("qscale", [0.5, 2.5, 8.0])
+@pytest.mark.parametrize("cap,bias,bidir", [(30.0, True, True), (30.0, False, False),
+                                            (0.0, True, True)])
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16)])
+def test_prefill_attention_capped_scores_of_every_size(qscale, cap, bias, bidir, d, dtype):
+    """Key tiles wholly before, around and wholly behind the rows, with scores below
+    a sixth of the cap, below half of it, and above."""
+    new, cached = [100, 300], [900, 100]
+    bd = [1000, 390] if bidir else None
+    c, lens = prefill_case(new, cached, 8, 2, d, 64, dtype, "hnd", cap, bias, bd, qscale=qscale)
+    run_prefill(c, new, lens, d, cap, bd)
+
+
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 1e-12])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (0.0, True), (20.0, True)])
+def test_prefill_attention_scales(scale, cap, bias):
+    new, cached = [70, 150], [300, 20]
+    c, lens = prefill_case(new, cached, 4, 2, 64, 16, F16, "hnd", cap, bias)
+    run_prefill(c, new, lens, 64, cap, scale=scale)
+
+
+@pytest.mark.parametrize("R", [31, 32, 33])
+def test_prefill_attention_batches_of_unequal_requests(R):
+    rng = random.Random(R)
+    new = [rng.choice([0, 1, 7, 64, 130]) for _ in range(R)]
+    cached = [rng.choice([0, 5, 128, 400, 900]) for _ in range(R)]
+    c, lens = prefill_case(new, cached, 7, 1, 64, 16, F16)
+    run_prefill(c, new, lens, 64)
 
 
 @pytest.mark.parametrize("d,dtype,ps,prefix,cap,bias,bidir", [
