@@ -85,8 +85,9 @@ def prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     requests share (pages ``prefix_pages`` int32; the prefix may end inside a
     page).  A row at position p attends the keys j of the prefix and of its own
     request with ``j <= p`` (and, with ``bidir`` int32 [R], the first ``bidir[r]``
-    own keys whatever its position); scores ``scale * q.k``, with ``softcap`` > 0 capped to ``softcap *
-    tanh(s / softcap)``, minus ``slopes[h] * |p - j|`` with ``slopes`` fp32 [Hq].
+    own keys whatever its position); scores ``scale * q.k``, with ``softcap`` > 0
+    capped to ``softcap * tanh(s / softcap)``, minus ``slopes[h] * |p - j|`` with
+    ``slopes`` fp32 [Hq].
     A row without keys is zero.  Rows of ``out`` behind ``cu_new[R]`` are left
     as they are.  Keys and values of a request must be finite; the rest of its
     last page may hold anything."""
@@ -108,6 +109,6 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     ``block_table[b]``; its query stands at position ``prefix_len + lens[b] - 1``.
     The prefix may end inside a page: the own keys start in pages of their own.
     ``softcap`` and ``slopes`` as in ``prefill_attention``.  A sequence without
-    keys gives zeros."""
+    keys gives zeros.  At most 8192 sequences."""
     return _lib.load_paged().decode_attention(q, k_pages, v_pages, block_table, lens, scale,
                                               prefix_pages, prefix_len, softcap, slopes, out)

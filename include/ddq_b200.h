@@ -476,6 +476,7 @@ int ddq_paged_prefill_attention(const void* q, int64_t q_token_stride, int64_t q
  * attention of a decode step (engine.py:225-251).  The query stands at position
  * prefix_len + lens[b] - 1; scores, mask and types as above.  prefix_pages may
  * be NULL with prefix_len 0.  A sequence without keys gives zeros.
+ * 1 <= B <= 8192.
  */
 int ddq_paged_decode_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                const ddq_paged_cache* cache, const int32_t* block_table,
