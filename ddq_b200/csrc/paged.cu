@@ -53,17 +53,19 @@ bool distinct(int64_t inner, const int64_t* n, const int64_t* st, int dims) {
 
 int check_attn(const void* q, int64_t q_ts, int64_t q_hs, const void* out, int64_t o_ts,
                int64_t o_hs, const int* table, int64_t table_stride, int64_t table_width,
-               const int* lens, float scale, float softcap, int64_t T, int64_t Hq, int64_t Hkv,
-               int64_t D) {
+               const int* lens, int64_t prefix_len, float scale, float softcap, int64_t T,
+               int64_t Hq, const PgCache& c) {
   if (!q || !out || !table || !lens) return DDQ_ERR_INVALID_ARGUMENT;
   if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.f)
     return DDQ_ERR_INVALID_ARGUMENT;
-  if (T > kIntMax || Hq < 1 || Hq > 1024 || Hq % Hkv != 0 || T * Hq > kIntMax || table_width < 1 ||
+  if (T > kIntMax || Hq < 1 || Hq > 1024 || Hq % c.Hkv != 0 || T * Hq > kIntMax || table_width < 1 ||
       table_width > kIntMax || table_stride < table_width || q_ts < 0 || o_ts < 0 || q_hs < 0 ||
       o_hs < 0)
     return DDQ_ERR_SHAPE;
+  // positions are 32-bit, up to a tile behind the last
+  if (prefix_len + (table_width << c.page_shift) > kIntMax - 255) return DDQ_ERR_SHAPE;
   const int64_t n[2] = {T, Hq}, st[2] = {o_ts, o_hs};
-  if (!distinct(D, n, st, 2)) return DDQ_ERR_SHAPE;
+  if (!distinct(c.D, n, st, 2)) return DDQ_ERR_SHAPE;
   if (!aligned16(q) || !aligned16(out) || q_ts % 8 != 0 || q_hs % 8 != 0 || o_ts % 8 != 0 ||
       o_hs % 8 != 0)
     return DDQ_ERR_ALIGNMENT;
@@ -133,7 +135,7 @@ PgParts make_parts(void* ws, int64_t rows, int64_t D, int count) {
   return PgParts{o, o + (size_t)count * rows * D, rows, 0, count};
 }
 bool attn_shape(int64_t T, int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
-                   int64_t page_size, int64_t prefix_len) {
+                int64_t page_size, int64_t prefix_len) {
   return T > 0 && R > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && D > 0 && table_width > 0 &&
          page_size > 0 && prefix_len >= 0;
 }
@@ -174,8 +176,8 @@ extern "C" int ddq_paged_prefill_attention(
   if (T == 0 || R == 0) return DDQ_OK;
   if (!cu_new || (prefix_len > 0 && !prefix_pages)) return DDQ_ERR_INVALID_ARGUMENT;
   st = check_attn(q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
-                  block_table, table_stride, table_width, lens, scale, softcap, T, Hq, c.Hkv,
-                  c.D);
+                  block_table, table_stride, table_width, lens, prefix_len, scale, softcap, T,
+                  Hq, c);
   if (st) return st;
   if (!(c.err = device_error_word())) return DDQ_ERR_DEVICE;
   const bool bf16 = cache->dtype == DDQ_DTYPE_BF16;
@@ -207,8 +209,8 @@ extern "C" int ddq_paged_decode_attention(
   if (B == 0) return DDQ_OK;
   if (prefix_len > 0 && !prefix_pages) return DDQ_ERR_INVALID_ARGUMENT;
   st = check_attn(q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
-                  block_table, table_stride, table_width, lens, scale, softcap, B, Hq, c.Hkv,
-                  c.D);
+                  block_table, table_stride, table_width, lens, prefix_len, scale, softcap, B,
+                  Hq, c);
   if (st) return st;
   const DcPlan plan = dc_plan(B, (int)Hq, c.Hkv, c.D, table_width << c.page_shift, prefix_len,
                               sm_count());

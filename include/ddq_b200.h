@@ -373,7 +373,8 @@ int ddq_unpack_argmax(const uint64_t* packed, int64_t M, int64_t* ids,
  * [page, g, row, d] of k and of v lies at page * page_stride + g * head_stride
  * + row * row_stride + d (strides in elements, multiples of 8; k and v 16-byte
  * aligned).  A table row lists a request's pages in order; entries past its
- * length are not read.  A page number, slot or position outside the pool (or
+ * length are not read; prefix_len + table_width * page_size stays below 2^31 - 255
+ * in the attention calls.  A page number, slot or position outside the pool (or
  * the rotary rows) is never followed: the write is left out, the attention of
  * that request (and of no other) is unspecified, and the device error word is
  * set to DDQ_ERR_PAGE.

@@ -85,6 +85,9 @@ def test_attention_refusals(lib):
         assert f(c=cache(ps=8)) == SHAPE and f(c=cache(d=80)) == SHAPE
         assert f(c=cache(dtype=0)) == INVALID
         assert f(plen=-1) == SHAPE and f(plen=5) == INVALID     # no prefix pages
+        # positions that 32 bits cannot hold
+        assert f(width=2 ** 27, stride=2 ** 27) == SHAPE
+        assert f(width=2 ** 26, stride=2 ** 26, prefix=A, plen=2 ** 30) == SHAPE
     assert pre(R=0) == OK and pre(R=-1) == SHAPE and pre(cu=None) == INVALID
 
 

@@ -3,7 +3,10 @@ the rotary embedding with the page write (bit for bit the fp32 form), prompt and
 decode attention against 64-bit forms with derived tolerances, their masks,
 lengths, layouts, bad pages, streams and graphs, and a run of them together."""
 import math
+import os
 import random
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -509,6 +512,35 @@ def test_results_do_not_change_from_call_to_call():
     for _ in range(5):
         assert torch.equal(run_decode(c, lens, prefix, 64), first)
         assert torch.equal(run_prefill(p, [300, 9], plens, 64), pf)
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing is initialised by a call in a way that a capture forbids."""
+    code = """
+import torch
+from ddq_b200 import paged
+i = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+kp, vp = (torch.zeros(8, 2, 16, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+cos, sin = torch.ones(64, 64, device="cuda"), torch.zeros(64, 64, device="cuda")
+qkv = torch.ones(5, 18 * 64, dtype=torch.float16, device="cuda")
+table, free, old, new, pre = i([-1] * 2, [-1] * 2), i(5, 2, 3), i(0, 0), i(4, 1), i(7)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    p = paged.plan_step(old, new, table, free, 16, 5, prefix_len=9)
+    q = paged.rope_kv_write(qkv, kp, vp, cos, sin, p.slots, p.positions, 14, 2, 64)
+    o = paged.prefill_attention(q, kp, vp, table, p.cu_new, p.lens, 0.125)
+    d = paged.decode_attention(q[3:], kp, vp, table, p.lens, 0.125, pre, 9)
+g.replay()
+torch.cuda.synchronize()
+assert table[:, 0].tolist() == [5, 2] and (o == 1).all() and (q == 1).all()
+# keys of ones (weight e^8) behind a prefix of zeros
+want = torch.tensor([n / (n + 9 * 2.718281828 ** -8) for n in (4, 1)], device="cuda")
+assert ((d.float() - want[:, None, None]).abs() < 2.0 ** -10).all()
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 def test_two_graphs_and_two_streams_share_nothing():
