@@ -344,7 +344,9 @@ __global__ void __launch_bounds__(TC_NT, 1)
   const int end_max = end_of((row0 + nrow - 1) / G);
   const int np = (min(P, end_max) + TC_KV - 1) / TC_KV;
   const int nt = np + (max(end_max - P, 0) + TC_KV - 1) / TC_KV;
-  const int lo = (int)((int64_t)nt * z / splits), cnt = (int)((int64_t)nt * (z + 1) / splits) - lo;
+  // (below 2^24 tiles in at most 64 parts)
+  const int lo = (int)((uint32_t)nt * (uint32_t)z / (uint32_t)splits),
+            cnt = (int)((uint32_t)nt * (uint32_t)(z + 1) / (uint32_t)splits) - lo;
   // tile k of this CTA: first key, keys that exist behind it, its list
   auto key0 = [&](int k) { return lo + k < np ? (lo + k) * TC_KV : P + (lo + k - np) * TC_KV; };
   auto limit = [&](int k) { return lo + k < np ? P : P + len; };
@@ -383,9 +385,9 @@ __global__ void __launch_bounds__(TC_NT, 1)
     const bool half_on = t < halves;
     // This warp's 32 rows of Q, K-major with the 128-byte swizzle, and later its
     // rows of the output, through the same shared memory (Q is done with when the
-    // last scores are there): D / 8 lanes read or write a row together.  (One
-    // thread per row touched 32 lines an access: 13 of 82 thousand cycles of a
-    // CTA of 16 tiles.)
+    // last scores are there): D / 8 lanes read or write a row together, all pieces in
+    // flight at once (loads into registers came back one after another: 9 thousand
+    // cycles instead of 3 for 256 rows of 128 elements).
     uint8_t* const rows = smem + t * L::TILE + (warp & 3) * 32 * 128;
     auto piece = [&](int row, int c) {  // 16-byte piece c of 64-element block 0
       return row * 128 + ((c ^ (row & 7)) << 4);
@@ -393,20 +395,15 @@ __global__ void __launch_bounds__(TC_NT, 1)
     {
       const int64_t q_off = real ? tok * a.q_ts + (int64_t)h * a.q_hs : -1;
       constexpr int LPR = D / 8;  // lanes per row
-      uint4 v[LPR];
 #pragma unroll
       for (int e = 0; e < LPR; ++e) {
         const int64_t off = __shfl_sync(0xffffffffu, q_off, e * (32 / LPR) + lane / LPR);
-        v[e] = make_uint4(0u, 0u, 0u, 0u);
-        if (off >= 0)
-          v[e] = *reinterpret_cast<const uint4*>(reinterpret_cast<const E*>(a.q) + off +
-                                                 8 * (lane % LPR));
-      }
-#pragma unroll
-      for (int e = 0; e < LPR; ++e) {
         const int row = e * (32 / LPR) + lane / LPR, c = lane % LPR;
-        *reinterpret_cast<uint4*>(rows + (c >> 3) * L::HB + piece(row, c & 7)) = v[e];
+        const E* src = reinterpret_cast<const E*>(a.q) + (off >= 0 ? off : 0) + 8 * c;
+        ptx::cp_async16_zfill(ptx::smem_u32(rows + (c >> 3) * L::HB + piece(row, c & 7)), src,
+                              off >= 0);
       }
+      ptx::cp_async_wait_all();
       ptx::fence_proxy_async_smem();
       tc_arrive(bar_q, lane);
     }
@@ -903,39 +900,38 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PgAttnArgs a, co
   if (row >= p.rows) return;
   const int t = (int)(row / a.Hq), h = (int)(row % a.Hq);
   if (a.cu && (t < a.cu[0] || t >= a.cu[a.R])) return;  // a padded row stays as it is
+  // four parts in flight together, the first ones while the maximum is found (a part
+  // without keys was not written: its values are dropped)
+  float v[4][DPL], ls[4];
+  auto load = [&](int z0) {
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int z = min(z0 + y, p.count - 1);
+      const float* src = p.o + (z * p.rows + row) * D + lane * DPL;
+      if constexpr (DPL == 2)
+        *reinterpret_cast<float2*>(v[y]) = *reinterpret_cast<const float2*>(src);
+      else
+        *reinterpret_cast<float4*>(v[y]) = *reinterpret_cast<const float4*>(src);
+      ls[y] = z0 + y < p.count ? p.lse[z * p.rows + row] : -INFINITY;
+    }
+  };
+  load(0);
   float mx = -INFINITY;
   for (int z = lane; z < p.count; z += 32) mx = fmaxf(mx, p.lse[z * p.rows + row]);
   mx = warp_max(mx);
   float den = 0.f, o[DPL];
 #pragma unroll
   for (int e = 0; e < DPL; ++e) o[e] = 0.f;
-  for (int z0 = 0; z0 < p.count; z0 += 32) {
-    const float ls = z0 + lane < p.count ? p.lse[(z0 + lane) * p.rows + row] : -INFINITY;
-    const float wl = ls == -INFINITY ? 0.f : exp2f(ls - mx);
-    const int m = min(32, p.count - z0);
-    for (int z1 = 0; z1 < m; z1 += 4) {  // four parts in flight
-      float v[4][DPL], w[4];
+  for (int z = 0; z < p.count;) {
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        w[y] = __shfl_sync(0xffffffffu, wl, (z1 + y) & 31);
-        if (z1 + y >= m) w[y] = 0.f;
+    for (int y = 0; y < 4; ++y) {
+      const float w = ls[y] == -INFINITY ? 0.f : exp2f(ls[y] - mx);
+      den += w;
 #pragma unroll
-        for (int e = 0; e < DPL; ++e) v[y][e] = 0.f;
-        if (w[y] != 0.f) {  // a part without keys was not written
-          const float* src = p.o + ((z0 + z1 + y) * p.rows + row) * D + lane * DPL;
-          if constexpr (DPL == 2)
-            *reinterpret_cast<float2*>(v[y]) = *reinterpret_cast<const float2*>(src);
-          else
-            *reinterpret_cast<float4*>(v[y]) = *reinterpret_cast<const float4*>(src);
-        }
-      }
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        den += w[y];
-#pragma unroll
-        for (int e = 0; e < DPL; ++e) o[e] = fmaf(w[y], v[y][e], o[e]);
-      }
+      for (int e = 0; e < DPL; ++e) o[e] = fmaf(w, w != 0.f ? v[y][e] : 0.f, o[e]);
     }
+    z += 4;
+    if (z < p.count) load(z);
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;  // NaN stays NaN
   E* dst = reinterpret_cast<E*>(a.out) + t * a.o_ts + (int64_t)h * a.o_hs + lane * DPL;
