@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
     }
     const int tiles = (cn * G + TC_ROWS - 1) / TC_ROWS;
     int s = 0;
+#pragma unroll 4
     for (int e = 0; e < a.R; ++e) {
       const int le = __shfl_sync(0xffffffffu, ln, e), te = __shfl_sync(0xffffffffu, tiles, e);
       if (le > ln || (le == ln && e <= lane)) s += te;
@@ -344,9 +345,11 @@ __global__ void __launch_bounds__(TC_NT, 1)
   const int end_max = end_of((row0 + nrow - 1) / G);
   const int np = (min(P, end_max) + TC_KV - 1) / TC_KV;
   const int nt = np + (max(end_max - P, 0) + TC_KV - 1) / TC_KV;
-  // (below 2^24 tiles in at most 64 parts)
-  const int lo = (int)((uint32_t)nt * (uint32_t)z / (uint32_t)splits),
-            cnt = (int)((uint32_t)nt * (uint32_t)(z + 1) / (uint32_t)splits) - lo;
+  int lo = 0, cnt = nt;
+  if (splits > 1) {  // (below 2^24 tiles in at most 64 parts)
+    lo = (int)((uint32_t)nt * (uint32_t)z / (uint32_t)splits);
+    cnt = (int)((uint32_t)nt * (uint32_t)(z + 1) / (uint32_t)splits) - lo;
+  }
   // tile k of this CTA: first key, keys that exist behind it, its list
   auto key0 = [&](int k) { return lo + k < np ? (lo + k) * TC_KV : P + (lo + k - np) * TC_KV; };
   auto limit = [&](int k) { return lo + k < np ? P : P + len; };
@@ -717,9 +720,9 @@ __global__ void __launch_bounds__(TC_NT, 1)
     ptx::reg_dec<TC_REG_ISSUE>();
     if (warp == 8) {
     // -------------------------------------------------------------------- TMA
-    const int br = min(1 << a.c.page_shift, TC_KV);   // rows of a box
-    const int nb = TC_KV / br;                        // boxes per tile and 64 dimensions
-    const int box = lane % nb, dh = lane / nb;        // this lane's
+    static_assert(TC_KV == 1 << 7, "boxes of a tile by shifts");
+    const int bs = min(a.c.page_shift, 7), br = 1 << bs;           // rows of a box
+    const int box = lane & ((TC_KV >> bs) - 1), dh = lane >> (7 - bs);  // this lane's
     const int* own = a.table + (int64_t)r * a.table_stride;
     int g_ring = 0;
     // page number and row of this lane's box of tile k (looked up a tile ahead:
