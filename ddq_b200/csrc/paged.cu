@@ -189,7 +189,7 @@ extern "C" int ddq_paged_prefill_attention(
   const PgParts parts = make_parts(workspace, T * Hq, c.D, splits);
   PgAttnArgs a{c, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
                block_table, table_stride, (int)table_width, lens, cu_new, bidir, prefix_pages,
-               (int)prefix_len, slopes, scale, softcap, (int)T, (int)R, (int)Hq};
+               (int)prefix_len, slopes, scale, softcap, (int)T, (int)R, (int)Hq, (int)Hq / c.Hkv};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   st = launch_paged_tc(a, bf16, parts, splits, wait_timeout_ns(), debug_flags(), s);
   if (st || splits == 1) return st;
@@ -219,7 +219,7 @@ extern "C" int ddq_paged_decode_attention(
   if (!(c.err = device_error_word())) return DDQ_ERR_DEVICE;
   PgAttnArgs a{c, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
                block_table, table_stride, (int)table_width, lens, nullptr, nullptr, prefix_pages,
-               (int)prefix_len, slopes, scale, softcap, (int)B, (int)B, (int)Hq};
+               (int)prefix_len, slopes, scale, softcap, (int)B, (int)B, (int)Hq, (int)Hq / c.Hkv};
   return launch_paged_decode(a, cache->dtype == DDQ_DTYPE_BF16, workspace, plan,
                              wait_timeout_ns(), debug_flags(), reinterpret_cast<cudaStream_t>(stream));
 }

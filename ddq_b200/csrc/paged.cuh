@@ -39,6 +39,7 @@ struct PgAttnArgs {
   const float* slopes;      // [Hq] or null
   float scale, cap;
   int T, R, Hq;
+  int G;                    // query heads of a key/value head
 };
 
 // Parts of a split key axis: part z of row t * Hq + h holds the row's output

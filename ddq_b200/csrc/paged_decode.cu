@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
                                   ~static_cast<uintptr_t>(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row4 = lane >> 2, col2 = 2 * (lane & 3);
-  const int G = a.Hq / a.c.Hkv, groups = dc_groups(G), segs = a.c.Hkv * groups;
+  const int G = a.G, groups = dc_groups(G), segs = a.c.Hkv * groups;
   const bool prefix = a.prefix_len > 0;
   if (tid == 0) {
     for (int s = 0; s < DC_NW * DC_SLOTS; ++s) ptx::mbar_init(ptx::smem_u32(&sm.full[s]), 1);
@@ -206,8 +206,8 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
     }
     const int seg = (int)dc_div(u0 - at, n);
     sm.start[w][0] = b;
-    sm.start[w][1] = seg / groups;
-    sm.start[w][2] = seg % groups;
+    sm.start[w][1] = groups == 1 ? seg : seg / groups;
+    sm.start[w][2] = groups == 1 ? 0 : seg % groups;
     sm.start[w][3] = (int)(u0 - at - (long long)seg * n);
     sm.start[w][4] = len;
     sm.start[w][5] = n;
@@ -237,8 +237,8 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
   const int count = (int)(uq + (worker < ur ? 1 : 0));
 
   // ---- loads: chunk after chunk of this warp, the page numbers one ahead
-  const int br = min(1 << a.c.page_shift, 32), nb = 32 / br;  // rows of a box, boxes of 32 keys
-  const int sub = lane % nb, dh = lane / nb;
+  const int bs = min(a.c.page_shift, 5), br = 1 << bs;      // rows of a box of the 32 keys
+  const int sub = lane & ((32 >> bs) - 1), dh = lane >> (5 - bs);
   const uint32_t ring = ptx::smem_u32(&sm.ring[warp * DC_SLOTS][0]);
   const uint32_t bar = ptx::smem_u32(&sm.full[warp * DC_SLOTS]);
   constexpr uint32_t SLOT = 32 * D * 2;
@@ -553,9 +553,9 @@ __global__ void __launch_bounds__(256)
   const int warp = threadIdx.x >> 5;
   const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;
   if (row >= (int64_t)a.T * a.Hq) return;
-  const int b = (int)(row / a.Hq), h = (int)(row % a.Hq);
-  const int G = a.Hq / a.c.Hkv, groups = dc_groups(G);
-  const int g = h / G, hh = h % G;
+  const int b = (int)((uint32_t)row / (uint32_t)a.Hq), h = (int)row - b * a.Hq;  // rows < 2^31
+  const int G = a.G, groups = dc_groups(G);
+  const int g = h / G, hh = h - g * G;
   const int2 ends = side.seg[((int64_t)b * a.c.Hkv + g) * groups + hh / 16];
   const bool split = ends.x != ends.y;
   if (!split && p.count == 0) return;  // written already

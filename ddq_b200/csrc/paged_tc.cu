@@ -201,7 +201,8 @@ __global__ void __launch_bounds__(TC_NT, 1)
   const uint32_t sbase = ptx::smem_u32(smem);
   __shared__ int found[6], wsum[TC_NT / 32];  // request, tile, first row, rows, keys, bidir
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int G = a.Hq / a.c.Hkv, g = blockIdx.x % a.c.Hkv, z = blockIdx.y;
+  const int tile0 = (int)(blockIdx.x / (unsigned)a.c.Hkv);
+  const int G = a.G, g = (int)blockIdx.x - tile0 * a.c.Hkv, z = blockIdx.y;
 
   const uint32_t bar_full = sbase + L::OFF_BAR;
   const uint32_t bar_empty = bar_full + 8 * L::ST;
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
   // last to the first and of up to 32 requests the longest is first (7679 tokens of 12
   // documents: 120 us; in the order of the batch 128, a head after the other 154; four
   // prompts of 4096 tokens: 504, a head after the other 514)
-  int r = 0, tile = blockIdx.x / a.c.Hkv, t_first = 0, n = a.T;
+  int r = 0, tile = tile0, t_first = 0, n = a.T;
   int len = 0, most = 0;  // own keys, and the ones that bidir lets every row attend
   if (a.cu && a.R <= 32) {  // each warp for itself: one round of loads, no barrier
     const int rr = a.R - 1 - lane;
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
     const int t = warp >> 2;
     const int rr = row0 + tid;                  // tid < 256: both halves in order
     const bool real = tid < nrow;
-    const int i = real ? rr / G : 0, h = g * G + (real ? rr % G : 0);
+    const int i = real ? (int)((unsigned)rr / (unsigned)G) : 0, h = g * G + (real ? rr - i * G : 0);
     const int tok = t_first + i;
     // a row behind the last takes part unmasked (its Q is zero, its result is not
     // stored): a warp of such rows has no slower tiles than the others
@@ -900,8 +901,8 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PgAttnArgs a, co
   ptx::pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= p.rows) return;
-  const int t = (int)(row / a.Hq), h = (int)(row % a.Hq);
+  if (row >= p.rows) return;  // rows < 2^31
+  const int t = (int)((uint32_t)row / (uint32_t)a.Hq), h = (int)row - t * a.Hq;
   if (a.cu && (t < a.cu[0] || t >= a.cu[a.R])) return;  // a padded row stays as it is
   // four parts in flight together, the first ones while the maximum is found (a part
   // without keys was not written: its values are dropped)
@@ -1034,7 +1035,7 @@ int tc_splits(int64_t T, int64_t R, int Hq, int Hkv, int64_t keys, bool ragged, 
 
 int launch_paged_tc(const PgAttnArgs& a, bool bf16, const PgParts& parts, int splits,
                     unsigned long long tmo, int debug_flags, cudaStream_t s) {
-  const int G = a.Hq / a.c.Hkv;
+  const int G = a.G;
   const int64_t tiles = tc_tiles(a.T, a.R, G, a.cu != nullptr);
   if (tiles > 0x7fffffff / a.c.Hkv) return DDQ_ERR_SHAPE;
   CUtensorMap tk, tv;
