@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(TC_NT, 1)
   // ---- the request and the tile of this CTA, kv heads next to each other: the CTAs
   // that start last shall have the fewest keys, so the tiles of a request go from the
   // last to the first and of up to 32 requests the longest is first (7679 tokens of 12
-  // documents: 120 us; in the order of the batch 128, a head after the other 154; four
-  // prompts of 4096 tokens: 504, a head after the other 514)
+  // documents: in the order of the batch 8 us more, a head after the other 34; four
+  // prompts of 4096 tokens, 486 us: a head after the other 10)
   int r = 0, tile = tile0, t_first = 0, n = a.T;
   int len = 0, most = 0;  // own keys, and the ones that bidir lets every row attend
   if (a.cu && a.R <= 32) {  // each warp for itself: one round of loads, no barrier
@@ -385,7 +385,11 @@ __global__ void __launch_bounds__(TC_NT, 1)
     // stored): a warp of such rows has no slower tiles than the others
     const int end = real ? end_of(i) : 0x7fffffff;
     const int pos = a.cu ? P + len - n + i : P + pg_len(a, real ? tok : 0) - 1;
-    float m = -INFINITY, l = 0.f;
+    // A row's own key, at distance 0, keeps its final maximum above -cap: starting
+    // there, keys far off under a steep bias come out as zeros at once and do not
+    // raise the maximum tile by tile, rescaling O.
+    float m = SCORED && a.cap > 0.f && pos >= 0 ? -a.cap * 1.4426950408889634f : -INFINITY;
+    float l = 0.f;
     const bool half_on = t < halves;
     // This warp's 32 rows of Q, K-major with the 128-byte swizzle, and later its
     // rows of the output, through the same shared memory (Q is done with when the
@@ -474,7 +478,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
           // to log2 units, capped and biased.  Where the polynomial serves all scores of
           // the warp: in registers, below.  Otherwise 32 scores at a time and back to S,
           // so that this rarer code, with more of its values alive, does not take
-          // registers from the rest (all in registers it spilled: 202 us instead of 180
+          // registers from the rest (all in registers it spilled: 22 us more
           // for 7679 tokens of 12 packed documents, 128-wide heads).
           const float d0 = (float)(pos - j0);
           big = 0.f;
@@ -622,8 +626,8 @@ __global__ void __launch_bounds__(TC_NT, 1)
             // results a cycle and SM, is the narrower one (four prompts of 4096
             // tokens, 128-wide heads: none 597 us, 1/8 570, 1/4 561, 3/8 563;
             // where keys are masked all on the latter, for weights of exactly 0; capped
-            // or biased scores use the FMA pipe enough, 154 us for the documents above
-            // instead of 166)
+            // or biased scores use the FMA pipe enough, 12 us less for the documents
+            // above)
             if (decltype(poly)::value && (c & 6) == 4) {
               tc_un(tc_poly_exp2(y0, y1), y0, y1);
             } else {

@@ -244,6 +244,20 @@ def test_prefill_attention_capped_scores_of_every_size(qscale, cap, bias, bidir,
     run_prefill(c, new, lens, d, cap, bd)
 
 
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16)])
+def test_prefill_attention_capped_rows_before_position_zero(d, dtype):
+    """A bidirectional prefix shows keys to rows that stand before them and have no
+    key of their own, under a bias of hundreds; long rows with a steep bias."""
+    new, cached = [600, 40, 130], [0, 0, 2000]
+    bd = [1, 3, 0]
+    c, lens = prefill_case(new, cached, 8, 2, d, 32, dtype, "hnd", 20.0, True, bd)
+    lens = [1, 30, lens[2]]
+    c["lens"] = ints(lens)
+    o = run_prefill(c, new, lens, d, 20.0, bd)
+    v0 = c["vp"][int(c["table"][0, 0]), :, 0].repeat_interleave(4, 0)
+    assert torch.equal(o[:600], v0.expand(600, 8, d))
+
+
 @pytest.mark.parametrize("scale", [-0.125, 0.0, 1e-12])
 @pytest.mark.parametrize("cap,bias", [(0.0, False), (0.0, True), (20.0, True)])
 def test_prefill_attention_scales(scale, cap, bias):
