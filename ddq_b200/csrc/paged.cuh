@@ -42,6 +42,11 @@ struct PgAttnArgs {
   int G;                    // query heads of a key/value head
 };
 
+// tanh(y) = y P(y^2) for |y| <= 1/2: P the minimax polynomial of degree 4 of
+// tanh(sqrt u) / sqrt(u) on [0, 1/4] (Remez, relative error 2^-26).
+constexpr float PG_TANH0 = 0.999999987f, PG_TANH1 = -0.333330694f, PG_TANH2 = 0.133247793f,
+                PG_TANH3 = -0.0529860753f, PG_TANH4 = 0.0171350066f;
+
 // Parts of a split key axis: part z of row t * Hq + h holds the row's output
 // over its keys, o[z][row][D], and log2 of the sum of its weights, lse[z][row]
 // (-inf: no keys, o not written).  A kernel writes from part `first` on; o null:

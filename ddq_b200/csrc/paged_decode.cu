@@ -25,6 +25,8 @@
 // and the outputs of the same two heads.
 #include <cudaTypedefs.h>
 
+#include <cfloat>
+
 #include "launch.cuh"
 #include "paged.cuh"
 #include "sm100_ptx.cuh"
@@ -334,6 +336,40 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
     ko[e] = dc_swz(lane & 15, 2 * e + (lane >> 4));
     vo[e] = dc_swz((lane & 7) + 8 * (lane >> 4), 2 * e + ((lane >> 3) & 1));
   }
+  // Scores of a unit capped and biased, in log2 units; the query is `ahead` of its
+  // first key.  cap tanh(y), y = scale s / cap, is scale s P(y^2) up to |y| = 1/2 and
+  // cap - 2 cap / (exp(2 y) + 1) above: the latter alone is off by a few 2^-23 of the
+  // cap, which is not small against a score far below it (3 under a cap of 10^6 came
+  // out as 2.9).  Each score goes by its own size, whatever the ones beside it are.
+  auto score = [&](float (&sc)[2][NB][4], int ahead) {
+    auto each = [&](auto f) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int nbk = 0; nbk < NB; ++nbk)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            f(sc[mt][nbk][i], slope[nbk][i & 1], 16 * mt + row4 + 8 * (i >> 1));
+    };
+    const float kk = a.scale * LOG2E;
+    if (a.cap > 0.f) {
+      const float A = a.cap * LOG2E, ratio = fminf(fmaxf(a.scale / a.cap, -FLT_MAX), FLT_MAX);
+      bool large = false;
+      each([&](float& v, float, int) { large |= !(fabsf(v * ratio) <= 0.5f); });
+      large = __any_sync(0xffffffffu, large);
+      each([&](float& v, float, int) {
+        const float y = v * ratio, w = y * y;
+        const float p = fmaf(fmaf(fmaf(fmaf(PG_TANH4, w, PG_TANH3), w, PG_TANH2), w, PG_TANH1), w,
+                             PG_TANH0);
+        v = large && !(fabsf(y) <= 0.5f)
+                ? A - __fdividef(2.f * A, dc_exp2(y * (2.f * LOG2E)) + 1.f)
+                : v * kk * p;
+      });
+    } else {
+      each([&](float& v, float, int) { v *= kk; });
+    }
+    each([&](float& v, float sl, int key) { v = fmaf(-sl, (float)(ahead - key), v); });
+  };
   for (int u = 0; u < count; ++u) {
     const int h0 = cw.g * G + cw.grp * 16;  // first query head
     const int heads = min(16, G - cw.grp * 16);
@@ -377,6 +413,7 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
           }
         }
         give();
+        if (!plain) score(sc, cw.len - 1 - base);
         bool grow = false;
         float mx[NB][2];
 #pragma unroll
@@ -390,15 +427,6 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
               for (int y = 0; y < 2; ++y) {
                 float& v = sc[mt][nbk][2 * y + x];
                 const int key = 16 * mt + row4 + 8 * y;
-                if (!plain) {
-                  if (a.cap > 0.f) {  // cap - 2 cap / (exp(2 y / cap) + 1), as paged_tc.cu
-                    const float A = a.cap * LOG2E;
-                    v = A - __fdividef(2.f * A, dc_exp2(v * (2.f * LOG2E * a.scale / a.cap)) + 1.f);
-                  } else {
-                    v *= a.scale * LOG2E;
-                  }
-                  v = fmaf(-slope[nbk][x], (float)(cw.len - 1 - base - key), v);
-                }
                 v = key < have ? v * mul : -INFINITY;
                 mx[nbk][x] = fmaxf(mx[nbk][x], v);
               }

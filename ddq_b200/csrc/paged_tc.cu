@@ -425,14 +425,13 @@ __global__ void __launch_bounds__(TC_NT, 1)
       const float slope = SCORED && a.slopes ? a.slopes[h] * LOG2E : 0.f;
       const float r2 = SCORED && a.cap > 0.f ? (a.scale / a.cap) * (a.scale / a.cap) : 0.f;
       const float r8 = (r2 * r2) * (r2 * r2);
-      const TcF2 cap0 = tc_pk1(a.cap > 0.f ? kk * 0.999999987f : kk),
-                 cap1 = tc_pk1(kk * -0.333330694f * r2),
-                 cap2 = tc_pk1(kk * 0.133247793f * (r2 * r2)),
-                 cap3 = tc_pk1(kk * -0.0529860753f * (r2 * r2 * r2)),
-                 cap4 = tc_pk1(kk * 0.0171350066f * r8);
-      // |y| <= 1/2, y = scale s / cap: cap tanh(y) = scale s P(y^2), P the minimax
-      // polynomial of degree 4 of tanh(sqrt u) / sqrt(u) on [0, 1/4] (Remez, error
-      // 2^-26), its coefficients in powers of s^2; up to |y| = 1/6 of degree 2 (error
+      const TcF2 cap0 = tc_pk1(a.cap > 0.f ? kk * PG_TANH0 : kk),
+                 cap1 = tc_pk1(kk * PG_TANH1 * r2),
+                 cap2 = tc_pk1(kk * PG_TANH2 * (r2 * r2)),
+                 cap3 = tc_pk1(kk * PG_TANH3 * (r2 * r2 * r2)),
+                 cap4 = tc_pk1(kk * PG_TANH4 * r8);
+      // |y| <= 1/2, y = scale s / cap: cap tanh(y) = scale s P(y^2), the coefficients in
+      // powers of s^2; up to |y| = 1/6 the minimax polynomial of degree 2 (error
       // 2^-24.7): six or four packed operations for two scores, their bias added, and no
       // special function.  Without a cap P is 1.
       auto capped_poly = [&](TcF2 x) {

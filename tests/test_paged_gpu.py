@@ -707,3 +707,83 @@ def test_a_serving_run(dtype, hq, hkv, d, ps, prefix, cap, bias):
             want, tol = expect(qr[r:r + 1], hist_k[r], hist_v[r],
                                torch.tensor([L - 1], device="cuda"))
             close(o[r:r + 1], want, tol)
+
+
+# --------------------------------------------- what scores and weights may be off
+def strict(q, k, v, pos, least, scale, cap, slope, w):
+    """As ``paged_reference.attend_many``, with a bound that does not grow with the cap.
+
+    softcap * tanh(s / softcap) is a function of s whose relative error, evaluated in
+    32 bits, is a few 2^-23 whatever the cap, so a score z is off by at most 2^-20 |z|
+    (and by the dot product's (D + 2) 2^-23 sum|q k| scale; 2^-20 also for the exponential).
+    w: how far a weight is off, relative to it, on its way to the weighted sum."""
+    n, d = q.shape
+    L = k.shape[0]
+    z = (q @ k.T) * scale
+    mag = (q.abs() @ k.abs().T).amax(1, keepdim=True) * abs(scale)
+    if cap:
+        z = cap * torch.tanh(z / cap)
+    j = torch.arange(L, device=q.device)[None, :]
+    if slope is not None:
+        z = z - slope * (pos[:, None] - j).abs().double()
+    keep = j < (pos + 1).clamp(min=least)[:, None]
+    z = torch.where(keep, z, torch.full_like(z, -math.inf))
+    p = torch.softmax(z, 1)
+    o, A = p @ v, p @ v.abs()
+    zmax = torch.where(keep, z.abs(), torch.zeros_like(z)).amax(1, keepdim=True)
+    e = (d + 2) * 2.0 ** -23 * mag + 2.0 ** -20 * zmax.clamp(min=1.0)
+    cnt = keep.sum(1, keepdim=True).double()
+    return o, (w + 2 * e + (cnt / 16 + 8) * 2.0 ** -22) * A + cnt * 2.0 ** -25 * v.abs().max()
+
+
+def strict_decode(c, lens, prefix, scale, cap, w):
+    """Every row of a decode case: the 64-bit results and their bounds."""
+    q, u = c["q"], torch.finfo(c["q"].dtype).eps / 2
+    B, hq, d = q.shape
+    hkv = c["kp"].shape[1]
+    o = torch.zeros(B, hq, d, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(o)
+    for b, n in enumerate(lens):
+        if prefix + n == 0:
+            continue
+        for h in range(hq):
+            g = h * hkv // hq
+            k = torch.cat([ref.rows_of(c["kp"], c["prefix"], prefix, g),
+                           ref.rows_of(c["kp"], c["table"][b], n, g)])
+            v = torch.cat([ref.rows_of(c["vp"], c["prefix"], prefix, g),
+                           ref.rows_of(c["vp"], c["table"][b], n, g)])
+            sl = c["slopes"][h].double() if c["slopes"] is not None else None
+            x, t = strict(q[b:b + 1, h].double(), k, v,
+                          torch.tensor([prefix + n - 1], device="cuda"), 0, scale, cap, sl, w)
+            o[b, h], tol[b, h] = x[0], (1 + u) * (t + u * x.abs())[0]
+    return o, tol
+
+
+@pytest.mark.parametrize("cap", [50.0, 1e3, 1e4, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("d,dtype,hq,hkv,prefix,bias", [
+    (64, F16, 14, 2, 0, False), (128, BF16, 16, 1, 0, True), (64, F16, 8, 2, 40, True)])
+def test_decode_attention_keeps_small_scores_under_a_large_cap(cap, d, dtype, hq, hkv, prefix,
+                                                               bias):
+    """Scores of a few units, far below the cap: the cap leaves them as they are."""
+    from ddq_b200 import paged
+    lens = [3, 9, 1, 40]
+    c = decode_case(lens, prefix, hq, hkv, d, 16, dtype, bias=bias, qscale=2.0)
+    o = paged.decode_attention(c["q"], c["kp"], c["vp"], c["table"], c["lens"], d ** -0.5,
+                               prefix_pages=c["prefix"], prefix_len=prefix, softcap=cap,
+                               slopes=c["slopes"])
+    want, tol = strict_decode(c, lens, prefix, d ** -0.5, cap, torch.finfo(dtype).eps / 2)
+    close(o, want, tol)
+
+
+def test_decode_attention_small_scores_beside_some_above_a_large_cap():
+    """A sequence, a head and single keys whose scores exceed half the cap, next to small ones."""
+    from ddq_b200 import paged
+    lens, cap = [30, 40, 35], 1e6
+    c = decode_case(lens, 0, 8, 1, 64, 16, BF16)
+    c["q"][0, 3] *= 1e6
+    c["kp"][int(c["table"][1, 0]), 0, 5] *= -1e7
+    o = paged.decode_attention(c["q"], c["kp"], c["vp"], c["table"], c["lens"], 0.125,
+                               softcap=cap)
+    want, tol = strict_decode(c, lens, 0, 0.125, cap, torch.finfo(BF16).eps / 2)
+    tol[1] = 1e30       # (sums of 1e7 in that sequence's scores)
+    close(o, want, tol)
