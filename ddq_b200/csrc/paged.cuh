@@ -47,6 +47,25 @@ struct PgAttnArgs {
 constexpr float PG_TANH0 = 0.999999987f, PG_TANH1 = -0.333330694f, PG_TANH2 = 0.133247793f,
                 PG_TANH3 = -0.0529860753f, PG_TANH4 = 0.0171350066f;
 
+// A capped score in log2 units, A tanh(y) with y = ratio v = kk v / A: by the
+// polynomial up to |y| = 1/2 and, where `large`, as A - 2 A / (exp(2 y) + 1)
+// above.  The latter alone is off by a few 2^-23 of the cap, which is not small
+// against a score far below it (3 under a cap of 10^6 came out as 2.9).
+__device__ __forceinline__ float pg_capped(float v, float kk, float ratio, float A, bool large) {
+  const float y = v * ratio, w = y * y;
+  const float p =
+      fmaf(fmaf(fmaf(fmaf(PG_TANH4, w, PG_TANH3), w, PG_TANH2), w, PG_TANH1), w, PG_TANH0);
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y * 2.885390082f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.f));
+  return large && !(fabsf(y) <= 0.5f) ? fmaf(-2.f * A, r, A) : v * kk * p;
+}
+
+// scale / cap, finite also under the smallest cap, so that a score of 0 stays 0
+__device__ __forceinline__ float pg_cap_ratio(float scale, float cap) {
+  return fminf(fmaxf(scale / cap, -3.4e38f), 3.4e38f);
+}
+
 // Parts of a split key axis: part z of row t * Hq + h holds the row's output
 // over its keys, o[z][row][D], and log2 of the sum of its weights, lse[z][row]
 // (-inf: no keys, o not written).  A kernel writes from part `first` on; o null:

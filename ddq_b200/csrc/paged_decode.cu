@@ -25,8 +25,6 @@
 // and the outputs of the same two heads.
 #include <cudaTypedefs.h>
 
-#include <cfloat>
-
 #include "launch.cuh"
 #include "paged.cuh"
 #include "sm100_ptx.cuh"
@@ -337,10 +335,7 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
     vo[e] = dc_swz((lane & 7) + 8 * (lane >> 4), 2 * e + ((lane >> 3) & 1));
   }
   // Scores of a unit capped and biased, in log2 units; the query is `ahead` of its
-  // first key.  cap tanh(y), y = scale s / cap, is scale s P(y^2) up to |y| = 1/2 and
-  // cap - 2 cap / (exp(2 y) + 1) above: the latter alone is off by a few 2^-23 of the
-  // cap, which is not small against a score far below it (3 under a cap of 10^6 came
-  // out as 2.9).  Each score goes by its own size, whatever the ones beside it are.
+  // first key.
   auto score = [&](float (&sc)[2][NB][4], int ahead) {
     auto each = [&](auto f) {
 #pragma unroll
@@ -353,18 +348,11 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
     };
     const float kk = a.scale * LOG2E;
     if (a.cap > 0.f) {
-      const float A = a.cap * LOG2E, ratio = fminf(fmaxf(a.scale / a.cap, -FLT_MAX), FLT_MAX);
+      const float A = a.cap * LOG2E, ratio = pg_cap_ratio(a.scale, a.cap);
       bool large = false;
       each([&](float& v, float, int) { large |= !(fabsf(v * ratio) <= 0.5f); });
       large = __any_sync(0xffffffffu, large);
-      each([&](float& v, float, int) {
-        const float y = v * ratio, w = y * y;
-        const float p = fmaf(fmaf(fmaf(fmaf(PG_TANH4, w, PG_TANH3), w, PG_TANH2), w, PG_TANH1), w,
-                             PG_TANH0);
-        v = large && !(fabsf(y) <= 0.5f)
-                ? A - __fdividef(2.f * A, dc_exp2(y * (2.f * LOG2E)) + 1.f)
-                : v * kk * p;
-      });
+      each([&](float& v, float, int) { v = pg_capped(v, kk, ratio, A, large); });
     } else {
       each([&](float& v, float, int) { v *= kk; });
     }

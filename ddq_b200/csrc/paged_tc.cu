@@ -74,12 +74,6 @@ __device__ __forceinline__ float tc_exp2(float x) {
   return y;
 }
 
-__device__ __forceinline__ float tc_rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ void tc_sts(uint32_t p, uint32_t a, uint32_t b, uint32_t c,
                                        uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d)
@@ -485,7 +479,8 @@ __global__ void __launch_bounds__(TC_NT, 1)
           for (int c = 0; c < 128; c += 2) big = tc_max3(big, fabsf(s[c]), fabsf(s[c + 1]));
           poly = __all_sync(0xffffffffu, big <= poly_max);
           if (!poly) {
-            const float k2 = a.cap > 0.f ? 2.f * kk / a.cap : 0.f, A = a.cap * LOG2E;
+            const float ratio = a.cap > 0.f ? pg_cap_ratio(a.scale, a.cap) : 0.f;
+            const float A = a.cap * LOG2E;
 #pragma unroll 1
             for (int c0 = 0; c0 < TC_KV; c0 += 32) {
               uint32_t o[32];
@@ -494,12 +489,10 @@ __global__ void __launch_bounds__(TC_NT, 1)
               tc_regs(o);
               float* x = reinterpret_cast<float*>(o);
               const float dc = d0 - (float)c0;
-              if (a.cap > 0.f) {
-                // cap tanh(y) = cap - 2 cap / (exp(2 y) + 1): an absolute error of a
-                // few 2^-23 cap, also where the exponential overflows
+              if (a.cap > 0.f) {  // each score by its own size: rows of small ones
+                // beside one above half the cap keep their value
 #pragma unroll
-                for (int c = 0; c < 32; ++c)
-                  x[c] = fmaf(-2.f * A, tc_rcp(tc_exp2(x[c] * k2) + 1.f), A);
+                for (int c = 0; c < 32; ++c) x[c] = pg_capped(x[c], kk, ratio, A, true);
               } else {
 #pragma unroll
                 for (int c = 0; c < 32; ++c) x[c] *= kk;

@@ -787,3 +787,40 @@ def test_decode_attention_small_scores_beside_some_above_a_large_cap():
     want, tol = strict_decode(c, lens, 0, 0.125, cap, torch.finfo(BF16).eps / 2)
     tol[1] = 1e30       # (sums of 1e7 in that sequence's scores)
     close(o, want, tol)
+
+
+@pytest.mark.parametrize("cap", [50.0, 1e3, 1e4, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("bias", [False, True])
+def test_prefill_attention_small_scores_beside_some_above_a_large_cap(cap, bias):
+    """Rows whose scores exceed half the cap among rows of small scores."""
+    from ddq_b200 import paged
+    new, cached = [40], [10]
+    c, lens = prefill_case(new, cached, 8, 1, 64, 16, BF16, "hnd", cap, bias)
+    c["q"][5, 2] *= 1e6
+    o = paged.prefill_attention(c["q"], c["kp"], c["vp"], c["table"], c["cu"], c["lens"], 0.125,
+                                softcap=cap, slopes=c["slopes"])
+    u = torch.finfo(BF16).eps / 2
+    k, v = ref.rows_of(c["kp"], c["table"][0], 50, 0), ref.rows_of(c["vp"], c["table"][0], 50, 0)
+    for h in range(8):
+        sl = c["slopes"][h].double() if bias else None
+        want, tol = strict(c["q"][:, h].double(), k, v, torch.arange(10, 50, device="cuda"), 0,
+                           0.125, cap, sl, u)
+        close(o[:, h], want, (1 + u) * (tol + u * want.abs()))
+
+
+@pytest.mark.parametrize("cap", [1e-3, 1e-30, 1e-39])
+def test_attention_under_a_tiny_cap(cap):
+    """Every score is the cap or nearly so, a score of 0 stays 0: all weights are equal."""
+    from ddq_b200 import paged
+    new, cached = [5, 40], [0, 100]
+    c, lens = prefill_case(new, cached, 8, 2, 64, 16, F16)
+    c["q"][3] = 0
+    o = paged.prefill_attention(c["q"], c["kp"], c["vp"], c["table"], c["cu"], c["lens"], 0.125,
+                                softcap=cap)
+    want, tol = ref.prefill_reference(c["q"], c["kp"], c["vp"], c["table"], new, lens, 0.125, cap,
+                                      None, None)
+    close(o, want, tol)
+    last = [4, 44]
+    o = paged.decode_attention(c["q"][last], c["kp"], c["vp"], c["table"], c["lens"], 0.125,
+                               softcap=cap)
+    close(o, want[last], tol[last])
