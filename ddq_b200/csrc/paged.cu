@@ -72,6 +72,25 @@ int check_attn(const void* q, int64_t q_ts, int64_t q_hs, const void* out, int64
   return DDQ_OK;
 }
 
+// A run of memory, and whether two of them, or one and a row of a table, share a byte.
+struct Span {
+  const void* p;
+  int64_t bytes;
+};
+
+bool meet(const Span& a, const Span& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes;
+}
+
+bool meets_row(const Span& a, const int32_t* table, int64_t stride, int64_t width, int64_t rows) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), t = reinterpret_cast<uintptr_t>(table);
+  const uintptr_t end = t + 4 * (uintptr_t)width;  // of the first row
+  // the first row that ends behind the start of a
+  const uintptr_t r = x < end ? 0 : (x - end) / (4 * (uintptr_t)stride) + 1;
+  return a.bytes > 0 && r < (uintptr_t)rows && t + r * 4 * (uintptr_t)stride < x + a.bytes;
+}
+
 }  // namespace
 }  // namespace ddq
 
@@ -84,14 +103,25 @@ extern "C" int ddq_plan_step(const int32_t* cached, const int32_t* new_tokens,
                              int32_t* cu_new, int32_t* lens, int64_t* slots, int64_t* positions,
                              int32_t* seq_ids, int32_t* free_head_out, int64_t R, int64_t T,
                              void* stream) {
-  if (R < 1 || T < 0 || table_width < 1 || table_stride < table_width || num_free < 0 ||
-      prefix_len < 0 || T > kIntMax || table_width > kIntMax || num_free > kIntMax ||
+  if (R < 1 || R > kPlanMaxR || T < 0 || table_width < 1 || table_stride < table_width ||
+      num_free < 0 || prefix_len < 0 || T > kIntMax || table_width > kIntMax || num_free > kIntMax ||
       page_shift_of(page_size) < 0)
     return DDQ_ERR_SHAPE;
   if (!cached || !new_tokens || !block_table || (num_free > 0 && !free_pages) || !cu_new ||
-      !lens || (T > 0 && (!slots || !positions || !seq_ids)) || !free_head_out ||
-      free_head == free_head_out)
+      !lens || (T > 0 && (!slots || !positions || !seq_ids)) || !free_head_out)
     return DDQ_ERR_INVALID_ARGUMENT;
+  // every CTA reads all of the inputs while others write: what is written lies apart
+  const Span mem[] = {{cu_new, 4 * (R + 1)}, {lens, 4 * R},      {slots, 8 * T},
+                      {positions, 8 * T},    {seq_ids, 4 * T},   {free_head_out, 4},
+                      {cached, 4 * R},       {new_tokens, 4 * R}, {free_pages, 4 * num_free},
+                      {free_head, free_head ? 4 : 0}};
+  constexpr int kWritten = 6;
+  for (int i = 0; i < (int)(sizeof(mem) / sizeof(mem[0])); ++i) {
+    if (meets_row(mem[i], block_table, table_stride, table_width, R))
+      return DDQ_ERR_INVALID_ARGUMENT;
+    for (int j = 0; j < i && j < kWritten; ++j)
+      if (meet(mem[i], mem[j])) return DDQ_ERR_INVALID_ARGUMENT;
+  }
   return launch_plan_step(cached, new_tokens, block_table, table_stride, (int)table_width,
                           free_pages, (int)num_free, free_head, page_shift_of(page_size),
                           prefix_len, cu_new, lens, slots, positions, seq_ids, free_head_out,

@@ -124,6 +124,7 @@ __device__ __forceinline__ int pg_check(const PgCache& c, int page) {
   return -1;
 }
 
+constexpr int kPlanMaxR = 8192;  // requests of a plan
 int launch_plan_step(const int* cached, const int* fresh, int* table, int64_t table_stride,
                      int width, const int* free_pages, int num_free, const int* free_head,
                      int page_shift, int64_t prefix_len, int* cu, int* lens, int64_t* slots,

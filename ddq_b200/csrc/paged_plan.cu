@@ -11,7 +11,7 @@
 //     slot = table[r, p / page] * page + p % page,  position = prefix_len + p
 //
 // One launch.  Both sums run over all requests, and a step has few of them
-// (at most PL_MAXR), so every CTA makes the whole scan itself in shared memory
+// (at most kPlanMaxR), so every CTA makes the whole scan itself in shared memory
 // (8 bytes a request, from L2 after the first CTA) instead of waiting for the
 // other CTAs' parts.  A token or a fresh page then finds its request by binary
 // search, so one long prompt among many short ones is spread over all threads;
@@ -24,7 +24,6 @@
 namespace ddq {
 
 constexpr int PL_NT = 512;
-constexpr int PL_MAXR = 8192;
 
 struct PlArgs {
   const int* cached;
@@ -161,7 +160,6 @@ int launch_plan_step(const int* cached, const int* fresh, int* table, int64_t ta
                      int page_shift, int64_t prefix_len, int* cu, int* lens, int64_t* slots,
                      int64_t* positions, int* seq_ids, int* free_head_out, int R, int T,
                      cudaStream_t s) {
-  if (R > PL_MAXR) return DDQ_ERR_SHAPE;
   const int sms = device_sm_count(current_device());
   if (sms <= 0) return DDQ_ERR_DEVICE;
   PlArgs a{cached, fresh, table, table_stride, width, free_pages, num_free, free_head,
@@ -171,7 +169,7 @@ int launch_plan_step(const int* cached, const int* fresh, int* table, int64_t ta
   const int smem = 2 * (R + 1) * (int)sizeof(int);
   static SmemAttrOnce attr;
   const int st = ensure_smem_attr(attr, current_device(), plan_step_kernel,
-                                  2 * (PL_MAXR + 1) * (int)sizeof(int));
+                                  2 * (kPlanMaxR + 1) * (int)sizeof(int));
   if (st) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);

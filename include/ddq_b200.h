@@ -405,7 +405,10 @@ typedef struct ddq_paged_cache {
  *   positions [T]     int64 prefix_len + index in the request; 0 behind the last
  *   seq_ids [T]       int32 request of the token; -1 behind the last
  *   free_head_out [1] free_head + pages taken (beyond num_free: that many are
- *                     missing); not the same memory as free_head
+ *                     missing)
+ * No output shares memory with another one, with an input or with a row of the
+ * table, nor an input with the table (DDQ_ERR_INVALID_ARGUMENT): lens in the
+ * place of cached, say, would be read back by other blocks.
  * T is the number of token rows of the step (a capacity: sum(new_tokens) <= T
  * is the caller's to keep; tokens past T are not written).  1 <= R <= 8192.
  */

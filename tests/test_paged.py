@@ -113,3 +113,31 @@ def test_plan_reference_by_hand():
     assert table == [[5, -1], [7, 9], [-1, -1]] and cu == [0, 2, 3, 3] and lens == [5, 17, 0]
     assert slots == [83, 84, 144, -1, -1] and pos == [103, 104, 116, 0, 0]
     assert seqs == [0, 0, 1, -1, -1] and at == 1
+
+
+def test_plan_step_refuses_outputs_over_what_other_blocks_read(lib):
+    """Every block reads all lengths while the first writes: lens in the place of cached
+    (or of new_tokens) gave slots and positions too large by the new tokens."""
+    R, T, width, stride, nfree = 3, 5, 8, 16, 4
+    size = dict(cached=4 * R, new=4 * R, free=4 * nfree, head=4, cu=4 * R + 4, lens=4 * R,
+                slots=8 * T, pos=8 * T, seq=4 * T, head_out=4)
+    home = {name: (1 << 20) + 0x1000 * i for i, name in enumerate([*size, "table"])}
+
+    def plan(**moved):
+        p = {**home, **moved}
+        return lib.ddq_plan_step(p["cached"], p["new"], p["table"], stride, width, p["free"],
+                                 nfree, p["head"], 16, 0, p["cu"], p["lens"], p["slots"],
+                                 p["pos"], p["seq"], p["head_out"], R, T, None)
+    written = ("cu", "lens", "slots", "pos", "seq", "head_out")
+    for name in written:
+        for other in size:
+            if other != name:   # at the same place; the ends overlapping by a word
+                assert plan(**{name: home[other]}) == INVALID
+                assert plan(**{name: home[other] + size[other] - 4}) == INVALID
+                assert plan(**{name: home[other] - size[name] + 4}) == INVALID
+    for name in size:           # a table row; its last word; the row before its first word
+        for row in range(R):
+            at = home["table"] + 4 * stride * row
+            assert plan(**{name: at}) == INVALID
+            assert plan(**{name: at + 4 * width - 4}) == INVALID
+            assert plan(**{name: at - size[name] + 4}) == INVALID

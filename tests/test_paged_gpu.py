@@ -824,3 +824,19 @@ def test_attention_under_a_tiny_cap(cap):
     o = paged.decode_attention(c["q"][last], c["kp"], c["vp"], c["table"], c["lens"], 0.125,
                                softcap=cap)
     close(o, want[last], tol[last])
+
+
+def test_step_plan_with_its_inputs_between_the_rows_of_the_table():
+    """One buffer a request row: pages, then other state; nothing of it is in the way."""
+    from ddq_b200 import paged
+    state = torch.full((2, 10), -1, dtype=torch.int32, device="cuda")
+    table, cached, new = state[:, :8], state[0, 8:], state[1, 8:]
+    cached.copy_(ints([3, 16])), new.copy_(ints([20, 1]))
+    table[0, 0], table[1, 0] = 5, 7
+    want = [row[:] for row in table.tolist()]
+    p = paged.plan_step(cached, new, table, ints([9, 8, 2]), 16, 21)
+    want, cu, lens, slots, pos, seqs, at = ref.plan_reference([3, 16], [20, 1], want, [9, 8, 2],
+                                                              16, 21, 0, 0)
+    assert table.tolist() == want and cached.tolist() == [3, 16] and new.tolist() == [20, 1]
+    assert p.cu_new.tolist() == cu and p.lens.tolist() == lens and p.slots.tolist() == slots
+    assert p.positions.tolist() == pos and p.free_head.tolist() == [at]
