@@ -255,10 +255,9 @@ __global__ void __launch_bounds__(TC_NT, 1)
       cn = a.cu[rr + 1] - c0;
       ln = a.lens[rr];
       if (a.bidir) bd = a.bidir[rr];
-      if (c0 < 0 || c0 >= a.T || cn < 0) cn = 0;
-      cn = min(cn, a.T - c0);
+      if (c0 < 0 || c0 >= a.T || cn < 0) c0 = cn = 0;
     }
-    const int tiles = (cn * G + TC_ROWS - 1) / TC_ROWS;
+    const int tiles = (min(cn, a.T - c0) * G + TC_ROWS - 1) / TC_ROWS;
     int s = 0;
 #pragma unroll 4
     for (int e = 0; e < a.R; ++e) {
@@ -287,10 +286,9 @@ __global__ void __launch_bounds__(TC_NT, 1)
         cn = a.cu[rr + 1] - c0;
         ln = a.lens[rr];
         if (a.bidir) bd = a.bidir[rr];
-        if (c0 < 0 || c0 >= a.T || cn < 0) cn = 0;
-        cn = min(cn, a.T - c0);
+        if (c0 < 0 || c0 >= a.T || cn < 0) c0 = cn = 0;
       }
-      const int tiles = (cn * G + TC_ROWS - 1) / TC_ROWS;
+      const int tiles = (min(cn, a.T - c0) * G + TC_ROWS - 1) / TC_ROWS;
       int s = tiles;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -330,7 +328,9 @@ __global__ void __launch_bounds__(TC_NT, 1)
   }
   const int P = a.prefix_len;
   const int least = a.cu ? (a.bidir ? P + min(most, len) : 0) : P;
-  const int row0 = tile * TC_ROWS, nrow = min(TC_ROWS, n * G - row0);
+  // n new tokens, the last of them without a row where q ends before cu does: the rows
+  // that exist keep their positions
+  const int row0 = tile * TC_ROWS, nrow = min(TC_ROWS, min(n, a.T - t_first) * G - row0);
   const int halves = nrow > TC_HALF ? 2 : 1;
   // keys of the row of token i: those below end(i); the last row has the most
   auto end_of = [&](int i) {

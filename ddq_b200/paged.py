@@ -89,7 +89,8 @@ def prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     capped to ``softcap * tanh(s / softcap)``, minus ``slopes[h] * |p - j|`` with
     ``slopes`` fp32 [Hq].
     A row without keys is zero.  Rows of ``out`` behind ``cu_new[R]`` are left
-    as they are.  Keys and values of a request must be finite; the rest of its
+    as they are; where ``cu_new`` exceeds T (a step planned with too few token
+    rows) the rows that exist keep their positions.  Keys and values of a request must be finite; the rest of its
     last page may hold anything."""
     return _lib.load_paged().prefill_attention(q, k_pages, v_pages, block_table, cu_new, lens,
                                                scale, softcap, slopes, bidir, prefix_pages,

@@ -452,7 +452,8 @@ size_t ddq_paged_decode_attention_workspace_size(int64_t B, int64_t Hq, int64_t 
  *   q, out  [T, Hq, D] of the cache's type, token and head strides in elements
  *           (multiples of 8, 16-byte aligned)
  *   cu_new  int32 [R + 1]: rows cu_new[r] .. cu_new[r + 1] - 1 are request r's
- *           (its last ones); rows behind cu_new[R] are left as they are
+ *           (its last ones); rows behind cu_new[R] are left as they are; where
+ *           cu_new exceeds T the rows that exist keep their positions
  *   lens    int32 [R]: keys of the request, its new tokens included
  *   bidir   int32 [R] or NULL; slopes fp32 [Hq] or NULL; softcap 0: none
  *   prefix_pages  int32 [ceil(prefix_len / page_size)] or NULL: prefix_len keys

@@ -840,3 +840,19 @@ def test_step_plan_with_its_inputs_between_the_rows_of_the_table():
     assert table.tolist() == want and cached.tolist() == [3, 16] and new.tolist() == [20, 1]
     assert p.cu_new.tolist() == cu and p.lens.tolist() == lens and p.slots.tolist() == slots
     assert p.positions.tolist() == pos and p.free_head.tolist() == [at]
+
+
+@pytest.mark.parametrize("extra", [0, 40])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (20.0, True)])
+def test_prefill_attention_of_a_request_cut_by_the_rows_of_q(extra, cap, bias):
+    """A step whose last request has more new tokens than q has rows (plan_step gives such
+    sums where num_tokens is too small): the rows that exist keep their positions."""
+    from ddq_b200 import paged
+    new, cached = [0] * extra + [4, 300], [0] * extra + [30, 100]
+    c, lens = prefill_case(new, cached, 8, 2, 64, 16, F16, "hnd", cap, bias)
+    want, tol = ref.prefill_reference(c["q"], c["kp"], c["vp"], c["table"], new, lens, 0.125, cap,
+                                      c["slopes"], None)
+    for T in (5, 104, 303):
+        o = paged.prefill_attention(c["q"][:T], c["kp"], c["vp"], c["table"], c["cu"], c["lens"],
+                                    0.125, softcap=cap, slopes=c["slopes"])
+        close(o, want[:T], tol[:T])
