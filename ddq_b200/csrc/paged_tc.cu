@@ -799,7 +799,23 @@ __global__ void __launch_bounds__(TC_NT, 1)
       ptx::mma_commit_if(who, bar_empty + 8 * s);
       if (halves_u == 1) ptx::mma_commit_if(who, bar_empty + 8 * s);
     };
-    auto qk = [&](int s) {  // K in stage s
+    // zeros in the rows of stage s behind the first `have`, which may hold anything (or
+    // were not loaded); both halves' warps write them, each before its own MMAs
+    auto clear = [&](int s, int have) {
+      if (have >= TC_KV) return;
+      uint8_t* rows = smem + L::OFF_RING + s * L::TILE;
+      for (int x = have * 8 + lane; x < TC_KV * 8; x += 32)
+#pragma unroll
+        for (int hb = 0; hb < D / 64; ++hb)
+          *reinterpret_cast<uint4*>(rows + hb * L::HB + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+    };
+    // K of tile k in stage s.  Scores behind the last key are masked, but how capped ones
+    // are computed goes by the largest of a warp's (above): what lies behind a request
+    // must not change the bits of its rows.
+    auto qk = [&](int k, int s) {
+      if (SCORED) clear(s, limit(k) - key0(k));
       const uint64_t b0 = dk + (uint64_t)(s * (L::TILE >> 4));
 #pragma unroll
       for (int e = 0; e < D / 16; ++e)
@@ -815,25 +831,14 @@ __global__ void __launch_bounds__(TC_NT, 1)
       wait(bar_sfree, 0);
       ptx::tc_fence_after();
     }
-    qk(0);
+    qk(0, 0);
     int sk = 2 % L::ST, sv = 1;       // stages of K of the next tile and V of this one
     uint32_t phk = 0, phv = 0, par = 0;
 #pragma unroll 1
     for (int k = 0; k < cnt_u; ++k, par ^= 1u) {
       wait(bar_full + 8 * sv, phv);
-      const int have = limit(k) - key0(k);
-      if (have < TC_KV) {
-        // V's rows behind the last key may hold anything (or were not loaded):
-        // their weights are zero, and 0 x NaN is NaN.  (Both halves' warps write
-        // the zeros, each before its own MMAs.)
-        uint8_t* vs = smem + L::OFF_RING + sv * L::TILE;
-        for (int x = have * 8 + lane; x < TC_KV * 8; x += 32)
-#pragma unroll
-          for (int hb = 0; hb < D / 64; ++hb)
-            *reinterpret_cast<uint4*>(vs + hb * L::HB + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-        ptx::fence_proxy_async_smem();
-        __syncwarp();
-      }
+      // V's rows behind the last key: their weights are zero, and 0 x NaN is NaN
+      clear(sv, limit(k) - key0(k));
       if (k + 1 < cnt_u) {
         wait(bar_full + 8 * sk, phk);
         // S is free once the other half has read it (half 1 of this tile; half 0 of
@@ -843,7 +848,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
         else
           wait(bar_sfree, par);
         ptx::tc_fence_after();
-        qk(sk);
+        qk(k + 1, sk);
       }
       const uint64_t b0 = dv + (uint64_t)(sv * (L::TILE >> 4));
       wait(bar_p + 8 * t, par);

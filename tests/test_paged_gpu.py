@@ -856,3 +856,18 @@ def test_prefill_attention_of_a_request_cut_by_the_rows_of_q(extra, cap, bias):
         o = paged.prefill_attention(c["q"][:T], c["kp"], c["vp"], c["table"], c["cu"], c["lens"],
                                     0.125, softcap=cap, slopes=c["slopes"])
         close(o, want[:T], tol[:T])
+
+
+@pytest.mark.parametrize("new,cached", [([20], [11]), ([3, 300], [0, 7])])
+def test_capped_scores_do_not_depend_on_what_lies_behind_a_request(new, cached):
+    """The same bits whatever the unused rows of the last page hold."""
+    from ddq_b200 import paged
+    c, lens = prefill_case(new, cached, 14, 2, 64, 16, F16, "hnd", 30.0, True)
+    outs = []
+    for fill in (0.0, 1e4, float("nan"), -60000.0):
+        for r, n in enumerate(lens):
+            if n % 16:
+                c["kp"][int(c["table"][r, n // 16]), :, n % 16:] = fill
+        outs.append(paged.prefill_attention(c["q"], c["kp"], c["vp"], c["table"], c["cu"],
+                                            c["lens"], 0.125, softcap=30.0, slopes=c["slopes"]))
+    assert all(torch.equal(o, outs[0]) for o in outs[1:])
