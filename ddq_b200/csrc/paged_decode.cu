@@ -444,7 +444,10 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
             }
           }
         }
-        uint32_t pb[2][NB][2];  // P^T of 16 keys: B fragments
+        // P^T of 16 keys: B fragments.  A weight goes to the sum in two parts, rounded and
+        // the rest (22 or 16 bits of it), as the dense cache's kernel for 64-wide heads
+        // passes it on: the tensor pipe is idle nine tenths of the time here.
+        uint32_t pb[2][NB][2], pl[2][NB][2];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -455,8 +458,12 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
             const float p2 = dc_exp2(sc[mt][nbk][2] - m0), p3 = dc_exp2(sc[mt][nbk][3] - m1);
             l[nbk][0] += p0 + p2;
             l[nbk][1] += p1 + p3;
-            pb[mt][nbk][0] = dc_transpose(Ty::pack(p0, p1));
-            pb[mt][nbk][1] = dc_transpose(Ty::pack(p2, p3));
+            const uint32_t h0 = Ty::pack(p0, p1), h1 = Ty::pack(p2, p3);
+            const float2 f0 = Ty::to_f2(h0), f1 = Ty::to_f2(h1);
+            pb[mt][nbk][0] = dc_transpose(h0);
+            pb[mt][nbk][1] = dc_transpose(h1);
+            pl[mt][nbk][0] = dc_transpose(Ty::pack(p0 - f0.x, p1 - f0.y));
+            pl[mt][nbk][1] = dc_transpose(Ty::pack(p2 - f1.x, p3 - f1.y));
           }
         take();
         if (!dead) {
@@ -479,6 +486,9 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
 #pragma unroll
               for (int nbk = 0; nbk < NB; ++nbk)
                 dc_mma<E>(o[e][nbk], r, pb[mt][nbk][0], pb[mt][nbk][1]);
+#pragma unroll
+              for (int nbk = 0; nbk < NB; ++nbk)
+                dc_mma<E>(o[e][nbk], r, pl[mt][nbk][0], pl[mt][nbk][1]);
             }
           give();
         }

@@ -90,8 +90,12 @@ def prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     ``slopes`` fp32 [Hq].
     A row without keys is zero.  Rows of ``out`` behind ``cu_new[R]`` are left
     as they are; where ``cu_new`` exceeds T (a step planned with too few token
-    rows) the rows that exist keep their positions.  Keys and values of a request must be finite; the rest of its
-    last page may hold anything."""
+    rows) the rows that exist keep their positions.  Keys and values of a request
+    must be finite; the rest of its last page may hold anything.
+
+    Scores and softmax statistics are fp32; a weight is rounded once to the type of
+    the pages on its way to the weighted sum (``ddq_b200.h`` says how exact the rest
+    is)."""
     return _lib.load_paged().prefill_attention(q, k_pages, v_pages, block_table, cu_new, lens,
                                                scale, softcap, slopes, bidir, prefix_pages,
                                                prefix_len, out)
@@ -110,6 +114,7 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     ``block_table[b]``; its query stands at position ``prefix_len + lens[b] - 1``.
     The prefix may end inside a page: the own keys start in pages of their own.
     ``softcap`` and ``slopes`` as in ``prefill_attention``.  A sequence without
-    keys gives zeros.  At most 8192 sequences."""
+    keys gives zeros.  At most 8192 sequences.  The weights of the own keys reach the
+    weighted sum in two parts (22 bits in fp16, 16 in bf16), those of the prefix in one."""
     return _lib.load_paged().decode_attention(q, k_pages, v_pages, block_table, lens, scale,
                                               prefix_pages, prefix_len, softcap, slopes, out)

@@ -460,9 +460,12 @@ size_t ddq_paged_decode_attention_workspace_size(int64_t B, int64_t Hq, int64_t 
  *           in front of every request's own (stored once; it may end inside a page)
  * Row i of n, at position p = prefix_len + len - n + i, attends the keys j of
  * the prefix and of its request with j < max(p + 1, prefix_len + min(bidir,
- * len)), score softcap * tanh(scale q.k / softcap) - slope |p - j|, softmax in
- * fp32; a row without keys is zero.  The keys and values of a request must be
- * finite; what lies behind them is not looked at.
+ * len)), score softcap * tanh(scale q.k / softcap) - slope |p - j|; a row without
+ * keys is zero.  Scores, maximum, sum and result are held in fp32; exponentials are
+ * good to 2^-18, and a weight is rounded once to the cache's type (11 bits of it in
+ * fp16, 8 in bf16) on its way to the weighted sum, not in the sum that divides it.
+ * The keys and values of a request must be finite; what lies behind them is not
+ * looked at.
  */
 int ddq_paged_prefill_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                 const ddq_paged_cache* cache, const int32_t* block_table,
@@ -479,8 +482,10 @@ int ddq_paged_prefill_attention(const void* q, int64_t q_token_stride, int64_t q
  * that all share (prefix_pages int32 [ceil(prefix_len / page_size)]), then the
  * sequence's own lens[b] keys in its own pages.  Takes the place of the
  * attention of a decode step (engine.py:225-251).  The query stands at position
- * prefix_len + lens[b] - 1; scores, mask and types as above.  prefix_pages may
- * be NULL with prefix_len 0.  A sequence without keys gives zeros.
+ * prefix_len + lens[b] - 1; scores, mask and types as above.  The weights of the
+ * own keys reach the weighted sum in two parts of the cache's type (22 or 16 bits),
+ * those of the prefix in one, as above.
+ * prefix_pages may be NULL with prefix_len 0.  A sequence without keys gives zeros.
  * 1 <= B <= 8192.
  */
 int ddq_paged_decode_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,

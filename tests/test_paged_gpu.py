@@ -871,3 +871,19 @@ def test_capped_scores_do_not_depend_on_what_lies_behind_a_request(new, cached):
         outs.append(paged.prefill_attention(c["q"], c["kp"], c["vp"], c["table"], c["cu"],
                                             c["lens"], 0.125, softcap=30.0, slopes=c["slopes"]))
     assert all(torch.equal(o, outs[0]) for o in outs[1:])
+
+
+@pytest.mark.parametrize("dtype,d,hq,hkv", [(F16, 64, 14, 2), (BF16, 128, 8, 2), (F16, 128, 16, 1),
+                                            (BF16, 64, 24, 2)])
+def test_decode_attention_weights_reach_the_sum_in_two_parts(dtype, d, hq, hkv):
+    """Values that cancel show a weight's rounding: two parts leave (u / 2)^2 or so of it."""
+    from ddq_b200 import paged
+    lens = [2, 4, 6, 30, 64, 33] * 4
+    c = decode_case(lens, 0, hq, hkv, d, 16, dtype)
+    c["q"][..., 4:] = 0                       # dot products of four exact products
+    c["vp"].fill_(1.0)
+    c["vp"][:, :, 1::2] = -1.0
+    o = paged.decode_attention(c["q"], c["kp"], c["vp"], c["table"], c["lens"], 0.125)
+    u = torch.finfo(dtype).eps / 2
+    want, tol = strict_decode(c, lens, 0, 0.125, 0.0, u * u)
+    close(o, want, tol)
