@@ -48,7 +48,9 @@ struct DcSide {
 template <int D>
 struct DcSmem {
   uint8_t ring[DC_NW * DC_SLOTS][32 * D * 2];
-  float out[DC_NW][8][D + 4];  // a warp's results of 8 heads on their way out
+  // a warp's results of 8 heads (4 where two CTAs shall fit) on their way out
+  static constexpr int HEADS = D == 64 ? 4 : 8;
+  float out[DC_NW][HEADS][D + 4];
   unsigned long long full[DC_NW * DC_SLOTS];
   long long wsum[DC_NW];
   int most[DC_NW];
@@ -104,7 +106,10 @@ __device__ __forceinline__ void dc_mma<__nv_bfloat16>(float* d, const uint32_t* 
 // byte offset of 16-byte piece j of row r in a tile of 64 elements a row
 __device__ __forceinline__ uint32_t dc_swz(int r, int j) { return r * 128 + ((j ^ (r & 7)) << 4); }
 
-// CTAs of an SM: shared memory (113 KB, 228 KB) and registers
+// CTAs of an SM, by registers and shared memory: 106 KB for 64-wide heads.  (With 8 heads
+// on their way out at a time it was 115 KB, two CTAs did not fit, and the units, shared
+// out for two an SM, ran as two waves: 64 sequences of 1 to 8192 keys, 14/2 heads of 64,
+// in 40 us instead of 34.)
 __host__ __device__ constexpr int dc_resident(int d, int nb) { return d == 64 && nb == 1 ? 2 : 1; }
 
 __host__ __device__ __forceinline__ int dc_groups(int G) { return (G + 15) / 16; }
@@ -530,27 +535,31 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
           pl[part_row(h)] = v == 0.f ? -INFINITY : m[nbk][x] + log2f(v);
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) {
-          sm.out[warp][col2 + x][16 * e + row4] = o[e][nbk][x] * inv;
-          sm.out[warp][col2 + x][16 * e + row4 + 8] = o[e][nbk][2 + x] * inv;
+          const int r = Sm::HEADS == 8 ? col2 + x : lane & 3;
+          sm.out[warp][r][16 * e + row4] = o[e][nbk][x] * inv;
+          sm.out[warp][r][16 * e + row4 + 8] = o[e][nbk][2 + x] * inv;
         }
-      }
-      __syncwarp();
-      for (int i = lane; i < min(8, heads - 8 * nbk) * (D / 8); i += 32) {
-        const int hr = i / (D / 8), h = 8 * nbk + hr, d = 8 * (i % (D / 8));
-        const float4 v = *reinterpret_cast<const float4*>(&sm.out[warp][hr][d]);
-        const float4 w = *reinterpret_cast<const float4*>(&sm.out[warp][hr][d + 4]);
-        if (direct) {
-          *reinterpret_cast<uint4*>(reinterpret_cast<E*>(a.out) + now.b * a.o_ts +
-                                    (int64_t)(h0 + h) * a.o_hs + d) =
-              make_uint4(Ty::pack(v.x, v.y), Ty::pack(v.z, v.w), Ty::pack(w.x, w.y),
-                         Ty::pack(w.z, w.w));
-        } else {
-          float* dst = po + part_row(h) * D + d;
-          *reinterpret_cast<float4*>(dst) = v;
-          *reinterpret_cast<float4*>(dst + 4) = w;
+        if (Sm::HEADS == 8 && x == 0) continue;
+        __syncwarp();
+        for (int i = lane; i < Sm::HEADS * (D / 8); i += 32) {
+          const int hr = i / (D / 8), d = 8 * (i % (D / 8));
+          const int h = 8 * nbk + (Sm::HEADS == 8 ? hr : 2 * hr + x);
+          if (h >= heads) break;
+          const float4 v = *reinterpret_cast<const float4*>(&sm.out[warp][hr][d]);
+          const float4 w = *reinterpret_cast<const float4*>(&sm.out[warp][hr][d + 4]);
+          if (direct) {
+            *reinterpret_cast<uint4*>(reinterpret_cast<E*>(a.out) + now.b * a.o_ts +
+                                      (int64_t)(h0 + h) * a.o_hs + d) =
+                make_uint4(Ty::pack(v.x, v.y), Ty::pack(v.z, v.w), Ty::pack(w.x, w.y),
+                           Ty::pack(w.z, w.w));
+          } else {
+            float* dst = po + part_row(h) * D + d;
+            *reinterpret_cast<float4*>(dst) = v;
+            *reinterpret_cast<float4*>(dst + 4) = w;
+          }
         }
+        __syncwarp();  // sm.out is free again
       }
-      __syncwarp();  // sm.out is free again
     }
   }
   if (dead) {         // copies in flight land before the shared memory goes
@@ -654,6 +663,9 @@ __global__ void __launch_bounds__(256)
 
 template <int D>
 constexpr int dc_smem_bytes() { return (int)sizeof(DcSmem<D>) + 1024; }
+// an SM has 228 KB for its CTAs, 1 KB of each CTA's its own
+static_assert(dc_resident(64, 1) * (dc_smem_bytes<64>() + 1024) <= 228 * 1024, "resident CTAs");
+static_assert(dc_resident(128, 1) * (dc_smem_bytes<128>() + 1024) <= 228 * 1024, "resident CTAs");
 
 // CTAs that fit the GPU at once.
 int dc_ctas(int64_t B, int Hq, int Hkv, int D, int64_t keys, int sms) {

@@ -887,3 +887,15 @@ def test_decode_attention_weights_reach_the_sum_in_two_parts(dtype, d, hq, hkv):
     u = torch.finfo(dtype).eps / 2
     want, tol = strict_decode(c, lens, 0, 0.125, 0.0, u * u)
     close(o, want, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,dtype,ps,prefix", [(14, 2, F16, 64, 0), (16, 2, BF16, 32, 100),
+                                                    (9, 3, F16, 256, 0)])
+def test_decode_attention_64_wide_with_units_for_two_blocks_an_sm(hq, hkv, dtype, ps, prefix):
+    """More units of 32 keys than one block on each SM has warps for, ranges that cut most
+    sequences, heads in groups of 3, 7 and 8."""
+    rng = random.Random(hq)
+    lens = [rng.choice([0, 1, 40, 1200, 2500, 1999]) for _ in range(48)]
+    c = decode_case(lens, prefix, hq, hkv, 64, ps, dtype)
+    o = run_decode(c, lens, prefix, 64)
+    assert torch.equal(run_decode(c, lens, prefix, 64), o)
