@@ -20,6 +20,7 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -108,10 +109,8 @@ def build_torch(force: bool = False) -> str:
     return TORCH_PATH
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library (and the paged operators' module) if needed; return
-    the library's path."""
-    build_torch(force)
+def build_library(force: bool = False, verbose: bool = False) -> str:
+    """Compile the library if needed; return its path."""
     if not force and not is_stale():
         return LIB_PATH
     os.makedirs(BUILD_DIR, exist_ok=True)
@@ -126,6 +125,19 @@ def build(force: bool = False, verbose: bool = False) -> str:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    """Compile the library and the paged operators' module if needed; return the
+    library's path.  The library needs neither Python's headers nor torch's: where
+    the module does not build, that is a warning, and only ``ddq_b200.paged``
+    raises (``build_torch`` does so itself)."""
+    path = build_library(force, verbose)
+    try:
+        build_torch(force)
+    except (RuntimeError, OSError) as e:
+        warnings.warn(f"ddq_b200.paged is not available: {e}", RuntimeWarning, stacklevel=2)
+    return path
 
 
 if __name__ == "__main__":
