@@ -10,7 +10,7 @@ import importlib.util
 import os
 import threading
 
-from .build import LIB_PATH, TORCH_PATH
+from .build import LIB_PATH, torch_path
 
 _c_int64 = ctypes.c_int64
 _vp = ctypes.c_void_p
@@ -136,11 +136,11 @@ def load_paged():
     lib = load()
     with _lock:
         if _paged is None:
-            if not os.path.exists(TORCH_PATH):
+            path = torch_path()  # (imports torch, whose libraries the module links against)
+            if not os.path.exists(path):
                 raise RuntimeError(
-                    f"ddq_b200: {TORCH_PATH} not found; build it with `python -m ddq_b200.build`")
-            import torch  # noqa: F401  (the libraries that the module links against)
-            spec = importlib.util.spec_from_file_location("_paged", TORCH_PATH)
+                    f"ddq_b200: {path} not found; build it with `python -m ddq_b200.build`")
+            spec = importlib.util.spec_from_file_location("_paged", path)
             mod = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(mod)
             mod.bind(*(ctypes.cast(getattr(lib, name), _vp).value for name in _PAGED_ENTRIES))

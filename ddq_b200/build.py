@@ -2,11 +2,12 @@
 
 Every ``csrc/*.cu`` file is compiled for sm_100a only
 (``-gencode arch=compute_100a,code=sm_100a``) with relocatable device code
-(but for WHOLE_PROGRAM), in parallel, then device-linked into one shared library that exports the C ABI
-declared in ``include/ddq_b200.h``.  The library links the CUDA runtime
-statically and does not depend on torch; ``_paged.so`` beside it, host code on
-torch's headers, holds the tensor checks of the paged operators.  Sources are rebuilt only when a
-``.cu``/``.cuh``/header file is newer than the library.
+(but for WHOLE_PROGRAM), in parallel, then device-linked into one shared library
+that exports the C ABI declared in ``include/ddq_b200.h``.  The library links the
+CUDA runtime statically and does not depend on torch; a module beside it, host
+code on torch's headers (``torch_path``), holds the tensor checks of the paged
+operators.  Sources are rebuilt only when a ``.cu``/``.cuh``/header file is newer
+than the library, or the module is not of this torch and Python.
 
     python -m ddq_b200.build            # build if stale
     python -m ddq_b200.build --force    # rebuild
@@ -31,7 +32,6 @@ LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libddq_b200.so")
 # the paged operators' checks and tensor handling as a CPython module on torch
 TORCH_SRC = os.path.join(CSRC, "torch_paged.cpp")
-TORCH_PATH = os.path.join(LIB_DIR, "_paged.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-rdc=true", "-Xcompiler", "-fPIC",
@@ -81,19 +81,33 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def torch_path() -> str:
+    """Where the paged operators' module for this torch and this Python lies: it is
+    compiled on torch's C++ classes and Python's C API, so a module of others is not
+    a module for these."""
+    import sysconfig
+
+    import torch
+    v = torch.version
+    tag = f"{torch.__version__}-{v.cuda}-{str(v.git_version)[:8]}"
+    tag += f"-cxx11abi{int(torch.compiled_with_cxx11_abi())}"
+    return os.path.join(LIB_DIR, f"_paged-{tag}{sysconfig.get_config_var('EXT_SUFFIX')}")
+
+
 def build_torch(force: bool = False) -> str:
     """The CPython module of the paged operators (host code only; it gets the
     library's entry points at run time)."""
+    path = torch_path()
     deps = [TORCH_SRC, os.path.abspath(__file__)] + glob.glob(os.path.join(INCLUDE, "*.h"))
-    if not force and os.path.exists(TORCH_PATH) and \
-            all(os.path.getmtime(TORCH_PATH) >= os.path.getmtime(p) for p in deps):
-        return TORCH_PATH
+    if not force and os.path.exists(path) and \
+            all(os.path.getmtime(path) >= os.path.getmtime(p) for p in deps):
+        return path
     import sysconfig
 
     import torch
     root = os.path.dirname(torch.__file__)
     os.makedirs(LIB_DIR, exist_ok=True)
-    tmp = TORCH_PATH + ".tmp"
+    tmp = f"{path}.{os.getpid()}.tmp"
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
@@ -105,8 +119,8 @@ def build_torch(force: bool = False) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for {TORCH_SRC}:\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, TORCH_PATH)
-    return TORCH_PATH
+    os.replace(tmp, path)
+    return path
 
 
 def build_library(force: bool = False, verbose: bool = False) -> str:

@@ -1,9 +1,11 @@
 """CPU tests of the build: what it compiles, and what it does where a part fails."""
 import os
+import sysconfig
 
 import pytest
+import torch
 
-from ddq_b200 import build as b
+from ddq_b200 import _lib, build as b
 
 
 def test_the_library_is_built_where_the_module_on_torch_does_not_build(monkeypatch, tmp_path):
@@ -20,3 +22,29 @@ def test_the_library_is_built_where_the_module_on_torch_does_not_build(monkeypat
     with pytest.warns(RuntimeWarning, match="ddq_b200.paged is not available: no Python.h"):
         assert b.build() == lib
     assert made == [True]
+
+
+@pytest.mark.parametrize("other", ["torch", "cuda", "source", "python"])
+def test_a_module_of_another_torch_or_python_is_not_taken(monkeypatch, other):
+    """The module is compiled on both's headers: it is neither fresh nor loaded elsewhere."""
+    b.build_torch()
+    here = b.torch_path()
+    assert os.path.exists(here)
+    if other == "torch":
+        monkeypatch.setattr(torch, "__version__", "9.9.9+cu999")
+    elif other == "cuda":
+        monkeypatch.setattr(torch.version, "cuda", "99.9")
+    elif other == "source":
+        monkeypatch.setattr(torch.version, "git_version", "f" * 40)
+    else:
+        monkeypatch.setattr(sysconfig, "get_config_var", lambda name: ".cpython-999.so")
+    assert b.torch_path() != here
+
+    def compiler(cmd, **kw):
+        raise OSError("the module would be compiled")
+    monkeypatch.setattr(b.subprocess, "run", compiler)
+    with pytest.raises(OSError, match="would be compiled"):
+        b.build_torch()
+    monkeypatch.setattr(_lib, "_paged", None)
+    with pytest.raises(RuntimeError, match="not found; build it"):
+        _lib.load_paged()
