@@ -60,16 +60,18 @@ def build(reference: str = DEFAULT_REFERENCE, force: bool = False) -> list[str]:
     """Build every module whose .so is missing or older than its source.
 
     Returns the list of built paths; returns [] without error when the
-    reference checkout is absent or empty (e.g. on the GPU box).
+    reference checkout is absent or empty (e.g. on the GPU box), and raises
+    where it has some of the sources but not all.
     """
-    if not os.path.isdir(reference):
+    sources = {name: os.path.join(reference, fname) for name, fname in MODULES.items()}
+    missing = [src for src in sources.values() if not os.path.exists(src)]
+    if len(missing) == len(sources):
         return []
+    if missing:
+        raise FileNotFoundError(f"incomplete reference checkout: {', '.join(missing)}")
     procs = []
-    for name, fname in MODULES.items():
-        src = os.path.join(reference, fname)
+    for name, src in sources.items():
         out = so_path(name)
-        if not os.path.exists(src):     # an empty or partial checkout
-            continue
         if not force and os.path.exists(out) and os.path.getmtime(out) >= os.path.getmtime(src):
             continue
         code = (f"import sys; sys.path.insert(0, {os.path.dirname(HERE)!r}); "

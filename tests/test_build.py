@@ -48,3 +48,21 @@ def test_a_module_of_another_torch_or_python_is_not_taken(monkeypatch, other):
     monkeypatch.setattr(_lib, "_paged", None)
     with pytest.raises(RuntimeError, match="not found; build it"):
         _lib.load_paged()
+
+
+def test_the_reference_modules_need_a_whole_checkout_or_none(monkeypatch, tmp_path):
+    """No checkout, or an empty one, is skipped; one that lacks a file is an error."""
+    from oracle import build_ref as r
+    monkeypatch.setattr(r, "REF_OUT", str(tmp_path / "out"))
+
+    def no_build(*a, **kw):
+        raise AssertionError("nothing is compiled here")
+    monkeypatch.setattr(r.subprocess, "Popen", no_build)
+    assert r.build(str(tmp_path / "absent")) == []
+    some = tmp_path / "checkout"
+    some.mkdir()
+    assert r.build(str(some)) == []
+    names = list(r.MODULES.values())
+    (some / names[1]).write_text("")
+    with pytest.raises(FileNotFoundError, match=names[0]):
+        r.build(str(some))
