@@ -51,10 +51,16 @@ bool distinct(int64_t inner, const int64_t* n, const int64_t* st, int dims) {
   return true;
 }
 
+// Index arrays (null: absent) on their natural alignment.
+template <typename... P>
+bool aligned_as(const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) % alignof(P) == 0) && ...);
+}
+
 int check_attn(const void* q, int64_t q_ts, int64_t q_hs, const void* out, int64_t o_ts,
                int64_t o_hs, const int* table, int64_t table_stride, int64_t table_width,
-               const int* lens, int64_t prefix_len, float scale, float softcap, int64_t T,
-               int64_t Hq, const PgCache& c) {
+               const int* lens, const int* prefix_pages, const float* slopes, int64_t prefix_len,
+               float scale, float softcap, int64_t T, int64_t Hq, const PgCache& c) {
   if (!q || !out || !table || !lens) return DDQ_ERR_INVALID_ARGUMENT;
   if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.f)
     return DDQ_ERR_INVALID_ARGUMENT;
@@ -67,7 +73,7 @@ int check_attn(const void* q, int64_t q_ts, int64_t q_hs, const void* out, int64
   const int64_t n[2] = {T, Hq}, st[2] = {o_ts, o_hs};
   if (!distinct(c.D, n, st, 2)) return DDQ_ERR_SHAPE;
   if (!aligned16(q) || !aligned16(out) || q_ts % 8 != 0 || q_hs % 8 != 0 || o_ts % 8 != 0 ||
-      o_hs % 8 != 0)
+      o_hs % 8 != 0 || !aligned_as(table, lens, prefix_pages, slopes))
     return DDQ_ERR_ALIGNMENT;
   return DDQ_OK;
 }
@@ -122,6 +128,9 @@ extern "C" int ddq_plan_step(const int32_t* cached, const int32_t* new_tokens,
     for (int j = 0; j < i && j < kWritten; ++j)
       if (meet(mem[i], mem[j])) return DDQ_ERR_INVALID_ARGUMENT;
   }
+  if (!aligned_as(cached, new_tokens, block_table, free_pages, free_head, cu_new, lens, slots,
+                  positions, seq_ids, free_head_out))
+    return DDQ_ERR_ALIGNMENT;
   return launch_plan_step(cached, new_tokens, block_table, table_stride, (int)table_width,
                           free_pages, (int)num_free, free_head, page_shift_of(page_size),
                           prefix_len, cu_new, lens, slots, positions, seq_ids, free_head_out,
@@ -143,7 +152,7 @@ extern "C" int ddq_paged_rope_kv(const void* qkv, int64_t qkv_stride,
   if (!distinct(c.D, n, pst, 3)) return DDQ_ERR_SHAPE;
   if (T > kIntMax || qkv_stride < (Hq + 2 * c.Hkv) * c.D) return DDQ_ERR_SHAPE;
   if (!aligned16(qkv) || qkv_stride % 8 != 0 || !aligned16(cos) || !aligned16(sin) ||
-      !aligned16(q_out))
+      !aligned16(q_out) || !aligned_as(slots, positions))
     return DDQ_ERR_ALIGNMENT;
   return launch_paged_rope_kv(qkv, qkv_stride, c, cache->dtype == DDQ_DTYPE_BF16, cos, sin,
                               max_pos, slots, positions, q_out, T, (int)Hq,
@@ -206,9 +215,10 @@ extern "C" int ddq_paged_prefill_attention(
   if (T == 0 || R == 0) return DDQ_OK;
   if (!cu_new || (prefix_len > 0 && !prefix_pages)) return DDQ_ERR_INVALID_ARGUMENT;
   st = check_attn(q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
-                  block_table, table_stride, table_width, lens, prefix_len, scale, softcap, T,
-                  Hq, c);
+                  block_table, table_stride, table_width, lens, prefix_pages, slopes, prefix_len,
+                  scale, softcap, T, Hq, c);
   if (st) return st;
+  if (!aligned_as(cu_new, bidir)) return DDQ_ERR_ALIGNMENT;
   if (!(c.err = device_error_word())) return DDQ_ERR_DEVICE;
   const bool bf16 = cache->dtype == DDQ_DTYPE_BF16;
   const int splits = tc_splits(T, R, (int)Hq, c.Hkv,
@@ -239,8 +249,8 @@ extern "C" int ddq_paged_decode_attention(
   if (B == 0) return DDQ_OK;
   if (prefix_len > 0 && !prefix_pages) return DDQ_ERR_INVALID_ARGUMENT;
   st = check_attn(q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
-                  block_table, table_stride, table_width, lens, prefix_len, scale, softcap, B,
-                  Hq, c);
+                  block_table, table_stride, table_width, lens, prefix_pages, slopes, prefix_len,
+                  scale, softcap, B, Hq, c);
   if (st) return st;
   const DcPlan plan = dc_plan(B, (int)Hq, c.Hkv, c.D, table_width << c.page_shift, prefix_len,
                               sm_count());

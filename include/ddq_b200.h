@@ -372,7 +372,8 @@ int ddq_unpack_argmax(const uint64_t* packed, int64_t M, int64_t* ids,
  * key/value heads of D = 64 or 128 dimensions, fp16 or bf16.  Element
  * [page, g, row, d] of k and of v lies at page * page_stride + g * head_stride
  * + row * row_stride + d (strides in elements, multiples of 8; k and v 16-byte
- * aligned).  A table row lists a request's pages in order; entries past its
+ * aligned; int32, int64 and fp32 arrays of all these calls on their natural
+ * alignment).  A table row lists a request's pages in order; entries past its
  * length are not read; prefix_len + table_width * page_size stays below 2^31 - 255
  * in the attention calls.  A page number, slot or position outside the pool (or
  * the rotary rows) is never followed: the write is left out, the attention of

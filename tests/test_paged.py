@@ -141,3 +141,38 @@ def test_plan_step_refuses_outputs_over_what_other_blocks_read(lib):
             assert plan(**{name: at}) == INVALID
             assert plan(**{name: at + 4 * width - 4}) == INVALID
             assert plan(**{name: at - size[name] + 4}) == INVALID
+
+
+def test_index_arrays_off_their_natural_alignment_are_refused(lib):
+    """An int64 read at a multiple of 4 (an int32 at one of 2) would fault on the device."""
+    four, two = (1 << 20) + 4, (1 << 20) + 2
+    names = ("cached", "new", "table", "free", "head", "cu", "lens", "slots", "pos", "seq",
+             "head_out")
+    home = {name: (2 << 20) + 0x1000 * i for i, name in enumerate(names)}
+
+    def plan(**moved):
+        p = {**home, **moved}
+        return lib.ddq_plan_step(p["cached"], p["new"], p["table"], 8, 8, p["free"], 4, p["head"],
+                                 16, 0, p["cu"], p["lens"], p["slots"], p["pos"], p["seq"],
+                                 p["head_out"], 3, 5, None)
+    for name in names:
+        assert plan(**{name: two}) == ALIGN
+    assert plan(slots=four) == ALIGN and plan(pos=four) == ALIGN
+
+    def rope(slots=A, pos=A):
+        return lib.ddq_paged_rope_kv(A, 18 * 64, cache(), A, A, 10, slots, pos, A, 3, 14, None)
+    assert rope(slots=four) == ALIGN and rope(pos=four) == ALIGN
+
+    def pre(table=A, cu=A, lens=A, bidir=None, prefix=None, plen=0, slopes=None):
+        return lib.ddq_paged_prefill_attention(A, 14 * 64, 64, cache(), table, 8, 8, cu, lens,
+                                               bidir, prefix, plen, slopes, 0.1, 0.0, A, 14 * 64,
+                                               64, 3, 2, 14, None, 0, None)
+
+    def dec(table=A, lens=A, prefix=None, plen=0, slopes=None):
+        return lib.ddq_paged_decode_attention(A, 14 * 64, 64, cache(), table, 8, 8, lens, prefix,
+                                              plen, slopes, 0.1, 0.0, A, 14 * 64, 64, 3, 14,
+                                              None, 0, None)
+    for f in (pre, dec):
+        assert f(table=two) == ALIGN and f(lens=two) == ALIGN and f(slopes=two) == ALIGN
+        assert f(prefix=two, plen=5) == ALIGN
+    assert pre(cu=two) == ALIGN and pre(bidir=two) == ALIGN
