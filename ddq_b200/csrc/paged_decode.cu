@@ -130,7 +130,8 @@ template <typename E, int D, int NB>
 __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
     paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const PgAttnArgs a,
-                        const PgParts parts, const DcSide side, const unsigned long long tmo) {
+                        const PgParts parts, const DcSide side, const unsigned long long tmo,
+                        const int never) {
   using Ty = PgType<E>;
   using Sm = DcSmem<D>;
   constexpr int H2 = D / 64;
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(DC_NW * 32, dc_resident(D, NB))
   auto issue = [&] {    // K or V of the unit looked up into the next slot
     if (!pend_v && pend_mine) pend_mine = pg_check(a.c, pend_page) >= 0;
     const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, pend_mine)) * br * 128u;
-    if (lane == 0) ptx::mbar_arrive_expect_tx(bar + 8 * is, bytes);
+    if (lane == 0) ptx::mbar_arrive_expect_tx(bar + 8 * is, bytes + never);
     __syncwarp();
     if (pend_mine)
       ptx::tma_load_4d(ring + is * SLOT + (uint32_t)(dh * 4096 + sub * br * 128),
@@ -725,7 +726,9 @@ int launch_paged_decode(const PgAttnArgs& a, bool bf16, void* ws, const DcPlan& 
     const int ast = ensure_smem_attr(once, dev, kern, smem);
     if (ast) return ast;
     cfg.dynamicSmemBytes = smem;
-    e = cudaLaunchKernelEx(&cfg, kern, tk, tv, a, parts, side, tmo);
+    // test hook (ddq_set_debug bit 0): 16 bytes that never come, so that the warps'
+    // bounded waits run out and they wind down
+    e = cudaLaunchKernelEx(&cfg, kern, tk, tv, a, parts, side, tmo, 16 * (debug_flags & 1));
     return DDQ_OK;
   };
   const bool wide = a.Hq / a.c.Hkv > 8;

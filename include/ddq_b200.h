@@ -509,8 +509,9 @@ int ddq_device_error(int* code, void* stream);
  * Test hook (no reference counterpart): set the limit of every device-side
  * bounded wait (0 = the 1 s default) and debug flags for later launches in
  * this process.  flags bit 0 makes the tensor-core decode and prefill
- * kernels (and the paged attention's) skip the accumulator-ready signal, so
- * their epilogue waits run out and report
+ * kernels (and the paged prompt attention's) skip the accumulator-ready signal
+ * (the paged decode kernel: expect 16 bytes more than it copies), so
+ * their bounded waits run out and report
  * DDQ_ERR_TIMEOUT through ddq_device_error() without faulting the GPU;
  * bit 1 turns on the phase trace read by ddq_read_trace(); bit 6 switches
  * on the opt-in 17..64-token tcgen05 resident-slice kernel, and bit 4 makes

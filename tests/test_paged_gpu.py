@@ -899,3 +899,23 @@ def test_decode_attention_64_wide_with_units_for_two_blocks_an_sm(hq, hkv, dtype
     c = decode_case(lens, prefix, hq, hkv, 64, ps, dtype)
     o = run_decode(c, lens, prefix, 64)
     assert torch.equal(run_decode(c, lens, prefix, 64), o)
+
+
+# ------------------------------------------- calls that the documentation allows
+@pytest.mark.parametrize("d,hq,hkv,prefix", [(64, 14, 2, 0), (128, 16, 1, 0), (64, 8, 2, 300)])
+def test_a_wait_of_the_decode_kernel_that_runs_out_is_reported(d, hq, hkv, prefix):
+    """A copy announced larger than it is (a test hook): the warps' bounded waits give up, the
+    kernel winds down, the device error word says so, and the next call is right."""
+    from ddq_b200 import _lib, paged
+    lens = [300, 0, 20, 700]
+    c = decode_case(lens, prefix, hq, hkv, d, 16, F16)
+    lib = _lib.load()
+    assert lib.ddq_set_debug(1, 2_000_000) == 0          # 2 ms
+    try:
+        paged.decode_attention(c["q"], c["kp"], c["vp"], c["table"], c["lens"], d ** -0.5,
+                               prefix_pages=c["prefix"], prefix_len=prefix)
+        torch.cuda.synchronize()
+    finally:
+        lib.ddq_set_debug(0, 0)
+    assert device_error() == 7                            # DDQ_ERR_TIMEOUT
+    run_decode(c, lens, prefix, d)
