@@ -428,7 +428,7 @@ int ddq_plan_step(const int32_t* cached, const int32_t* new_tokens, int32_t* blo
  *          (elements, multiple of 8)
  *   cos, sin  fp32 [max_pos, D]; positions int64 [T], slots int64 [T] (< 0: the
  *          row's k and v are not written; no slot twice)
- *   q_out  [T, Hq, D]: rope(q) of every row
+ *   q_out  [T, Hq, D]: rope(q) of every row; apart from qkv
  */
 int ddq_paged_rope_kv(const void* qkv, int64_t qkv_stride, const ddq_paged_cache* cache,
                       const float* cos, const float* sin, int64_t max_pos, const int64_t* slots,
@@ -451,7 +451,8 @@ size_t ddq_paged_decode_attention_workspace_size(int64_t B, int64_t Hq, int64_t 
  * their pages (which hold the new tokens' keys and values already).  Takes the
  * place of the prompt attention of engine.py:225-251.
  *   q, out  [T, Hq, D] of the cache's type, token and head strides in elements
- *           (multiples of 8, 16-byte aligned)
+ *           (multiples of 8, 16-byte aligned); out may be q itself, otherwise they
+ *           lie apart
  *   cu_new  int32 [R + 1]: rows cu_new[r] .. cu_new[r + 1] - 1 are request r's
  *           (its last ones); rows behind cu_new[R] are left as they are; where
  *           cu_new exceeds T the rows that exist keep their positions

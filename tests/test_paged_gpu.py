@@ -919,3 +919,47 @@ def test_a_wait_of_the_decode_kernel_that_runs_out_is_reported(d, hq, hkv, prefi
         lib.ddq_set_debug(0, 0)
     assert device_error() == 7                            # DDQ_ERR_TIMEOUT
     run_decode(c, lens, prefix, d)
+
+
+@pytest.mark.parametrize("prefix,cap", [(0, 0.0), (70, 20.0)])
+def test_prefill_attention_bidirectional_beyond_32_requests(prefix, cap):
+    rng = random.Random(5)
+    R = 70
+    new = [rng.choice([0, 1, 7, 30, 130]) for _ in range(R)]
+    cached = [rng.choice([0, 5, 128, 300]) for _ in range(R)]
+    bd = [rng.choice([0, 3, n + c, 10 ** 6]) for n, c in zip(new, cached)]
+    c, lens = prefill_case(new, cached, 8, 2, 64, 16, F16, "hnd", cap, bool(cap), bd,
+                           prefix=prefix)
+    run_prefill(c, new, lens, 64, cap, bd, prefix=prefix)
+
+
+@pytest.mark.parametrize("new,cached", [([200], [0]), ([512] * 4, [0] * 4), ([3, 90], [700, 40])])
+@pytest.mark.parametrize("width", [512, 8192])
+def test_prefill_attention_with_a_table_wider_than_the_requests(new, cached, width):
+    """A table for the longest context there may be: most parts of the key axis are empty."""
+    c, lens = prefill_case(new, cached, 14, 2, 64, 16, F16)
+    table = torch.full((len(new), width), -1, dtype=torch.int32, device="cuda")
+    table[:, :c["table"].shape[1]] = c["table"]
+    c["table"] = table
+    o = run_prefill(c, new, lens, 64)
+    assert torch.equal(run_prefill(c, new, lens, 64), o)
+
+
+@pytest.mark.parametrize("prefix", [0, 150])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_attention_into_its_own_queries(prefix, cap):
+    """out = q, for one part of the key axis and for several."""
+    for new, cached in (([300, 5], [0, 40]), ([20], [3000])):
+        c, lens = prefill_case(new, cached, 14, 2, 64, 16, F16, prefix=prefix, cap=cap)
+        want = run_prefill(c, new, lens, 64, cap, prefix=prefix)
+        from ddq_b200 import paged
+        paged.prefill_attention(c["q"], c["kp"], c["vp"], c["table"], c["cu"], c["lens"], 0.125,
+                                softcap=cap, prefix_pages=c["prefix"], prefix_len=prefix,
+                                out=c["q"])
+        assert torch.equal(c["q"], want)
+    lens = [3000, 1, 0, 40, 700]
+    c = decode_case(lens, prefix, 14, 2, 64, 16, F16)
+    want = run_decode(c, lens, prefix, 64, cap)
+    paged.decode_attention(c["q"], c["kp"], c["vp"], c["table"], c["lens"], 0.125,
+                           prefix_pages=c["prefix"], prefix_len=prefix, softcap=cap, out=c["q"])
+    assert torch.equal(c["q"], want)
