@@ -11,8 +11,8 @@ namespace {
 constexpr int64_t kIntMax = 0x7fffffff;
 
 int page_shift_of(int64_t page_size) {
-  for (int sh = 4; sh <= 8; ++sh)
-    if (page_size == (int64_t)1 << sh) return sh;
+  for (int sh = 0; (int64_t)1 << sh <= DDQ_PAGE_SIZE_MAX; ++sh)
+    if (page_size == (int64_t)1 << sh) return page_size >= DDQ_PAGE_SIZE_MIN ? sh : -1;
   return -1;
 }
 
@@ -169,9 +169,9 @@ size_t parts_bytes(int64_t rows, int64_t D, int count) {
   return count > 1 ? (size_t)count * rows * (D + 1) * sizeof(float) : 0;
 }
 PgParts make_parts(void* ws, int64_t rows, int64_t D, int count) {
-  if (count <= 1) return PgParts{nullptr, nullptr, rows, 0, 1};
+  if (count <= 1) return PgParts{nullptr, nullptr, rows, 1};
   float* o = static_cast<float*>(ws);
-  return PgParts{o, o + (size_t)count * rows * D, rows, 0, count};
+  return PgParts{o, o + (size_t)count * rows * D, rows, count};
 }
 bool attn_shape(int64_t T, int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
                 int64_t page_size, int64_t prefix_len) {

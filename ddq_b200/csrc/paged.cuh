@@ -68,21 +68,18 @@ __device__ __forceinline__ float pg_cap_ratio(float scale, float cap) {
 
 // Parts of a split key axis: part z of row t * Hq + h holds the row's output
 // over its keys, o[z][row][D], and log2 of the sum of its weights, lse[z][row]
-// (-inf: no keys, o not written).  A kernel writes from part `first` on; o null:
-// one part, written to the output itself.
+// (-inf: no keys, o not written).  o null: one part, written to the output itself.
 struct PgParts {
   float* o;
   float* lse;
   int64_t rows;
-  int first, count;
+  int count;
 };
 
 template <typename T>
 struct PgType;
 template <>
 struct PgType<__half> {
-  static __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-  static __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
   static __device__ __forceinline__ float2 to_f2(uint32_t u) {
     return __half22float2(*reinterpret_cast<const __half2*>(&u));
   }
@@ -93,8 +90,6 @@ struct PgType<__half> {
 };
 template <>
 struct PgType<__nv_bfloat16> {
-  static __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-  static __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
   static __device__ __forceinline__ float2 to_f2(uint32_t u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
   }

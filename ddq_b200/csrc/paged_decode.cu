@@ -696,7 +696,7 @@ int launch_paged_decode(const PgAttnArgs& a, bool bf16, void* ws, const DcPlan& 
   const int count = a.prefix_len ? plan.splits + 1 : 0;
   const PgParts parts{count ? reinterpret_cast<float*>(w) : nullptr,
                       count ? reinterpret_cast<float*>(w + plan.off_lse) : nullptr,
-                      (int64_t)a.T * a.Hq, 0, count};
+                      (int64_t)a.T * a.Hq, count};
   const DcSide side{reinterpret_cast<float*>(w + plan.off_so),
                     reinterpret_cast<float*>(w + plan.off_sl),
                     reinterpret_cast<int2*>(w + plan.off_seg)};

@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
     if (tid < nrow) {
       const int tok = t_first + (row0 + tid) / G, h = g * G + (row0 + tid) % G;
       if (parts.o) {
-        parts.lse[(int64_t)(parts.first + z) * parts.rows + (int64_t)tok * a.Hq + h] = -INFINITY;
+        parts.lse[(int64_t)z * parts.rows + (int64_t)tok * a.Hq + h] = -INFINITY;
       } else {
         E* dst = reinterpret_cast<E*>(a.out) + tok * a.o_ts + (int64_t)h * a.o_hs;
 #pragma unroll
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(TC_NT, 1)
     // the last, stores nothing.
     if (half_on) {
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: 0; NaN stays
-      const int64_t prow = (int64_t)(parts.first + z) * parts.rows + (int64_t)tok * a.Hq + h;
+      const int64_t prow = (int64_t)z * parts.rows + (int64_t)tok * a.Hq + h;
       const bool part = parts.o != nullptr;
       if (part && real) parts.lse[prow] = l == 0.f ? -INFINITY : m + log2f(l);
       // offset of this thread's row; -1: nothing to store

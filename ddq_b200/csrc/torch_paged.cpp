@@ -52,11 +52,11 @@ double real(PyObject* o) {
   return v;
 }
 
-bool page_size_ok(int64_t ps) {
-  return ps == 16 || ps == 32 || ps == 64 || ps == 128 || ps == 256;
+void check_page_size(int64_t ps, const char* what) {
+  TORCH_CHECK(ps >= DDQ_PAGE_SIZE_MIN && ps <= DDQ_PAGE_SIZE_MAX && (ps & (ps - 1)) == 0, what,
+              ": page_size must be a power of two from ", DDQ_PAGE_SIZE_MIN, " to ",
+              DDQ_PAGE_SIZE_MAX);
 }
-
-constexpr const char* kPageSizes = "page_size must be one of (16, 32, 64, 128, 256)";
 
 bool vec(const at::Tensor& t, at::ScalarType type, c10::Device dev) {
   return t.scalar_type() == type && t.device() == dev && t.dim() == 1 && t.is_contiguous();
@@ -84,7 +84,7 @@ Pool pool(const at::Tensor& k, const at::Tensor& v, const char* what) {
   TORCH_CHECK(v.scalar_type() == k.scalar_type() && v.device() == k.device() &&
                   v.sizes() == k.sizes(),
               what, ": k_pages and v_pages must have the same type and shape");
-  TORCH_CHECK(page_size_ok(k.size(2)), what, ": ", kPageSizes);
+  check_page_size(k.size(2), what);
   TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128, what, ": head_dim must be 64 or 128");
   const int64_t a = stride(k, 0), b = stride(k, 1), r = stride(k, 2);
   TORCH_CHECK(k.stride(3) == 1 && (a | b | r) % 8 == 0, what,
@@ -131,7 +131,7 @@ PyObject* plan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     head = h.data_ptr<int32_t>();
   }
   TORCH_CHECK(R >= 1, W, ": at least one request");
-  TORCH_CHECK(page_size_ok(ps), W, ": ", kPageSizes);
+  check_page_size(ps, W);
   TORCH_CHECK(T >= 0 && prefix >= 0, W, ": negative count");
   c10::cuda::OptionalCUDAGuard guard;
   if (dev.index() != c10::cuda::current_device()) guard.set_device(dev);

@@ -23,8 +23,6 @@ import torch
 
 from . import _lib
 
-PAGE_SIZES = (16, 32, 64, 128, 256)
-
 
 class StepPlan(NamedTuple):
     """What ``plan_step`` returns (device tensors)."""

@@ -368,7 +368,7 @@ int ddq_unpack_argmax(const uint64_t* packed, int64_t M, int64_t* ids,
  * reference's dense-cache path that it takes the place of.
  * ---------------------------------------------------------------------------
  *
- * A pool of num_pages pages of page_size rows (16, 32, 64, 128 or 256) for Hkv
+ * A pool of num_pages pages of page_size rows (a power of two, 16 to 256) for Hkv
  * key/value heads of D = 64 or 128 dimensions, fp16 or bf16.  Element
  * [page, g, row, d] of k and of v lies at page * page_stride + g * head_stride
  * + row * row_stride + d (strides in elements, multiples of 8; k and v 16-byte
@@ -380,6 +380,9 @@ int ddq_unpack_argmax(const uint64_t* packed, int64_t M, int64_t* ids,
  * that request (and of no other) is unspecified, and the device error word is
  * set to DDQ_ERR_PAGE.
  */
+#define DDQ_PAGE_SIZE_MIN 16
+#define DDQ_PAGE_SIZE_MAX 256
+
 typedef struct ddq_paged_cache {
   void* k;
   void* v;
