@@ -13,7 +13,7 @@
 // the joining kernel adds the parts up in order; there are no atomics, and no
 // warp waits for another one (with a CTA per range, its four warps joined at the
 // end of every sequence, 2048 segments of 0 to 511 keys, 128-wide heads, took 77 us
-// instead of 55; 40 sequences of 1 to 32768 keys take 276 us, 94% of a copy's rate).
+// instead of 55; 40 sequences of 1 to 32768 keys take 284 us, 92% of a copy's rate).
 //
 // Each warp has a ring of its own, K and V of a unit in turn, that TMA fills from
 // the pages, across the ends of sequences.  Per unit, on mma.sync m16n8k16 with the

@@ -14,7 +14,7 @@
 // pieces); a thread takes 8 dimensions of the first half of one or more heads
 // with the matching 8 of the second half - always the same dimensions, so that
 // the token's cos and sin stay in its registers for all its heads (32 bytes each
-// were read again for every head: 204 us instead of 135, 6.2 TB/s, for 32768 tokens
+// were read again for every head: 204 us instead of 137, 6.1 TB/s, for 32768 tokens
 // of 32 + 2 x 8 heads of 128) - and its 16-byte loads of all heads are in flight together.
 #include "launch.cuh"
 #include "paged.cuh"

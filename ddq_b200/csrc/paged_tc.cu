@@ -52,7 +52,8 @@ constexpr int TC_ROWS = 256;     // rows per CTA
 constexpr int TC_NT = 384;        // two softmax warpgroups and one for TMA and MMA issue
 // Registers a thread: launched with 168 (3 warps on each quarter of the SM);
 // the third warpgroup gives up 80, the softmax ones take 40 each: 256 x 208 +
-// 128 x 88 = 384 x 168.  A softmax thread holds its row of 128 scores.
+// 128 x 88 = 384 x 168.  A softmax thread holds its row of 128 scores (the plain
+// kernels spill 16 bytes at that, the scored ones nothing).
 constexpr int TC_REG_SOFTMAX = 208, TC_REG_ISSUE = 88;
 constexpr float TC_LAZY = 8.f;   // log2 units
 
@@ -1014,7 +1015,10 @@ int64_t tc_tiles(int64_t T, int64_t R, int64_t G, bool ragged) {
 // Splits of the key axis, where the CTAs would not fill the GPU: the number with the
 // least of rounds x (key tiles of a CTA + 3 for its start and end) plus the parts'
 // way through memory (a tile takes about 1.5 us, in which 9 MB pass) and, for
-// prompts, the joining kernel, which a decode step has anyway.
+// prompts, the joining kernel, which a decode step has anyway.  The keys are those
+// that the table's width could hold, for the lengths are on the device: with a table
+// much wider than the requests, short ones are split too (8 prompts of 512 tokens,
+// 20 us, take 51 with a table for 32768 keys).
 int tc_splits(int64_t T, int64_t R, int Hq, int Hkv, int64_t keys, bool ragged, int sms) {
   const int64_t ctas = tc_tiles(T, R, Hq / Hkv, ragged) * Hkv;
   const int64_t nt = (keys + TC_KV - 1) / TC_KV;

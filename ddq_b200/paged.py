@@ -82,16 +82,18 @@ def prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     ``block_table[r]`` lists; in front of them stand ``prefix_len`` keys that all
     requests share (pages ``prefix_pages`` int32; the prefix may end inside a
     page).  A row at position p attends the keys j of the prefix and of its own
-    request with ``j <= p`` (and, with ``bidir`` int32 [R], the first ``bidir[r]``
-    own keys whatever its position); scores ``scale * q.k``, with ``softcap`` > 0
-    capped to ``softcap * tanh(s / softcap)``, minus ``slopes[h] * |p - j|`` with
-    ``slopes`` fp32 [Hq].
+    request with ``j <= p`` (and, with ``bidir`` int32 [R], the prefix and the
+    first ``bidir[r]`` own keys whatever its position); scores ``scale * q.k``, with
+    ``softcap`` > 0 capped to ``softcap * tanh(s / softcap)``, minus
+    ``slopes[h] * |p - j|`` with ``slopes`` fp32 [Hq].
     A row without keys is zero.  Rows of ``out`` behind ``cu_new[R]`` are left
     as they are; where ``cu_new`` exceeds T (a step planned with too few token
     rows) the rows that exist keep their positions.  Keys and values of a request
     must be finite; the rest of its last page may hold anything.
 
-    Scores and softmax statistics are fp32; a weight is rounded once to the type of
+    The key axis is split by what ``block_table`` could hold: where the longest
+    request is known on the host, pass the columns that it uses
+    (``block_table[:, :n]``, no copy).  Scores and softmax statistics are fp32; a weight is rounded once to the type of
     the pages on its way to the weighted sum (``ddq_b200.h`` says how exact the rest
     is)."""
     return _lib.load_paged().prefill_attention(q, k_pages, v_pages, block_table, cu_new, lens,
